@@ -16,6 +16,7 @@ I32, I64 = 0, 1
 LOSS_BPR, LOSS_HINGE, LOSS_ADAPTIVE_BPR, LOSS_ADAPTIVE_HINGE, LOSS_WARP = range(5)
 OPT_SGD, OPT_ADAGRAD, OPT_SPARSE_ADAM, OPT_ADAM = range(4)
 SIDE_USER, SIDE_ITEM = 0, 1
+F32, BF16, F16 = 0, 1, 2
 MAX_META = 16
 MAX_NEG = 63
 
@@ -23,6 +24,8 @@ LOSS_KINDS = {'bpr': LOSS_BPR, 'hinge': LOSS_HINGE, 'adaptive_bpr': LOSS_ADAPTIV
               'adaptive_hinge': LOSS_ADAPTIVE_HINGE, 'warp': LOSS_WARP}
 OPT_ALGOS = {'sgd': OPT_SGD, 'adagrad': OPT_ADAGRAD, 'sparse_adam': OPT_SPARSE_ADAM,
              'adam': OPT_ADAM}
+ACTIVATIONS = {'identity': 0, 'relu': 1, 'leaky_relu': 2, 'sigmoid': 3, 'silu': 4, 'gelu': 5}
+ELEMENT_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 
 class CollieHipError(RuntimeError):
@@ -232,6 +235,37 @@ SIGNATURES = {
                                                 c_void_p, c_int64, POINTER(OptimCfg), c_void_p,
                                                 c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
                                                 c_void_p]),
+    'collie_embedding_rows': (ctypes.c_int, [c_void_p, c_int32, c_int64, c_int32, c_void_p, c_int32,
+                                             c_int64, c_float, c_void_p, c_void_p, c_void_p]),
+    'collie_embedding_rows_grad_workspace_bytes': (c_size_t, [c_int64, c_int32]),
+    'collie_embedding_rows_grad': (ctypes.c_int, [c_void_p, c_int32, c_int64, c_void_p, c_int64,
+                                                  c_int32, c_int64, c_int32, c_float, c_int64,
+                                                  c_void_p, c_void_p, c_size_t, c_void_p,
+                                                  c_void_p]),
+    'collie_layer_norm_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32,
+                                                 c_void_p, c_void_p, c_int32, c_float, c_void_p,
+                                                 c_void_p, c_void_p, c_void_p]),
+    'collie_layer_norm_backward_workspace_bytes': (c_size_t, [c_int64, c_int32]),
+    'collie_layer_norm_backward': (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                                  c_int64, c_int32, c_void_p, c_int32, c_void_p,
+                                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                  c_size_t, c_void_p]),
+    'collie_linear_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
+                                             c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                             c_void_p, c_void_p]),
+    'collie_gated_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
+                                            c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+                                            c_void_p, c_void_p, c_void_p]),
+    'collie_layer_backward_workspace_bytes': (c_size_t, [c_int32, c_int64, c_int32, c_int32,
+                                                         c_int32]),
+    'collie_linear_backward': (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64,
+                                              c_int32, c_void_p, c_int32, c_int32, c_void_p,
+                                              c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                              c_void_p]),
+    'collie_gated_backward': (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64,
+                                             c_int32, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -12,6 +12,9 @@ namespace collie {
 int sort_and_segment(const SortWs& s, int64_t nkeys, uint32_t split, hipStream_t stream,
                      uint32_t* seg_of = nullptr);
 
+// Only the sort (a workspace of carve_pair_sort_ws is enough).
+int sort_pairs(const SortWs& s, int64_t nkeys, hipStream_t stream);
+
 inline const uint32_t* sorted_keys(const SortWs& s, int64_t nkeys) {
   return s.keys[(radix_plan(nkeys).passes - 1) & 1];
 }

@@ -501,19 +501,20 @@ int run_pass(const SortWs& s, const uint32_t* kin, const uint32_t* vin, uint32_t
 
 }  // namespace
 
-int sort_and_segment(const SortWs& s, int64_t nkeys, uint32_t split, hipStream_t stream,
-                     uint32_t* seg_of) {
-  const RadixPlan plan = radix_plan(nkeys);
-  COLLIE_REQUIRE(plan.passes <= 4, "key range too large for the radix plan");
-  if (small_coalesce(s.m)) {
-    int nbits = 1;
-    while ((int64_t{1} << nbits) < nkeys) ++nbits;
-    const int out = (plan.passes - 1) & 1;  // where sorted_keys() / sorted_vals() look
-    hipLaunchKernelGGL(small_sort_segment_kernel, dim3(1), dim3(kSmallBlock), 0, stream, s.ekeys,
-                       s.ecodes, static_cast<int>(s.m), nbits, split, s.keys[out], s.vals[out],
-                       s.seg_start, s.nseg, s.long_base, seg_of);
-    return check_launch("small_sort_segment_kernel");
-  }
+namespace {
+
+// the one-workgroup form, in the buffers where sorted_keys() / sorted_vals() look
+int small_sort(const SortWs& s, int64_t nkeys, uint32_t split, hipStream_t stream, uint32_t* seg_of) {
+  int nbits = 1;
+  while ((int64_t{1} << nbits) < nkeys) ++nbits;
+  const int out = (radix_plan(nkeys).passes - 1) & 1;
+  hipLaunchKernelGGL(small_sort_segment_kernel, dim3(1), dim3(kSmallBlock), 0, stream, s.ekeys,
+                     s.ecodes, static_cast<int>(s.m), nbits, split, s.keys[out], s.vals[out],
+                     s.seg_start, s.nseg, s.long_base, seg_of);
+  return check_launch("small_sort_segment_kernel");
+}
+
+int radix_sort(const SortWs& s, const RadixPlan& plan, hipStream_t stream) {
   for (int pass = 0; pass < plan.passes; ++pass) {
     const uint32_t* kin = pass == 0 ? s.ekeys : s.keys[(pass - 1) & 1];
     const uint32_t* vin = pass == 0 ? s.ecodes : s.vals[(pass - 1) & 1];
@@ -527,6 +528,24 @@ int sort_and_segment(const SortWs& s, int64_t nkeys, uint32_t split, hipStream_t
     }
     if (rc) return rc;
   }
+  return 0;
+}
+
+}  // namespace
+
+int sort_pairs(const SortWs& s, int64_t nkeys, hipStream_t stream) {
+  const RadixPlan plan = radix_plan(nkeys);
+  COLLIE_REQUIRE(plan.passes <= 4, "key range too large for the radix plan");
+  if (small_coalesce(s.m)) return small_sort(s, nkeys, 0xffffffffu, stream, nullptr);
+  return radix_sort(s, plan, stream);
+}
+
+int sort_and_segment(const SortWs& s, int64_t nkeys, uint32_t split, hipStream_t stream,
+                     uint32_t* seg_of) {
+  const RadixPlan plan = radix_plan(nkeys);
+  COLLIE_REQUIRE(plan.passes <= 4, "key range too large for the radix plan");
+  if (small_coalesce(s.m)) return small_sort(s, nkeys, split, stream, seg_of);
+  if (const int rc = radix_sort(s, plan, stream)) return rc;
   const uint32_t* sorted = sorted_keys(s, nkeys);
   const dim3 grid(static_cast<unsigned>(s.ntiles));
   hipLaunchKernelGGL(seg_count_kernel, grid, dim3(kBlock), 0, stream, sorted, s.m, s.blk_heads);

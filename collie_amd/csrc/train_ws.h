@@ -114,6 +114,25 @@ inline void carve_sort_ws(Carver& c, SortWs& s, int64_t m, int D) {
   s.partial = c.take<float>(static_cast<size_t>(s.max_pieces) * (D + 1));
 }
 
+// what sort_pairs() (rowsort.h) needs: no segments, no pieces (the one-workgroup form of the sort
+// writes the segments of its few entries all the same)
+inline void carve_pair_sort_ws(Carver& c, SortWs& s, int64_t m) {
+  memset(&s, 0, sizeof(s));
+  s.m = m;
+  s.ntiles = (m + kSortTile - 1) / kSortTile;
+  s.ekeys = c.take<uint32_t>(m);
+  s.ecodes = c.take<uint32_t>(m);
+  for (int i = 0; i < 2; ++i) {
+    s.keys[i] = c.take<uint32_t>(m);
+    s.vals[i] = c.take<uint32_t>(m);
+  }
+  s.hist = c.take<uint32_t>((size_t{1} << kMaxRadixBits) * static_cast<size_t>(s.ntiles));
+  s.totals = c.take<uint32_t>(4 * (size_t{1} << kMaxRadixBits));
+  s.seg_start = c.take<uint32_t>(kSmallMax + 1);
+  s.nseg = c.take<uint32_t>(64);
+  s.long_base = c.take<uint32_t>(kSmallMax);
+}
+
 // radix plan for keys in [0, nkeys)
 struct RadixPlan {
   int passes;

@@ -1,27 +1,95 @@
 """
 Parameter containers of the MF model (reference: ``collie/model/base/layers.py``).
 
-They are ``torch.nn.Embedding`` subclasses only so that ``state_dict()`` keys, shapes, the
-``sparse`` flag and the initial distributions are those of the reference; their ``forward`` is not
-on the hot path (all lookups happen inside the HIP kernels, straight from ``.weight``).
+The tables are ``torch.nn.Embedding`` subclasses, so that ``state_dict()`` keys, shapes, the
+``sparse`` flag and the initial distributions are those of the reference.  The fused paths look rows
+up inside their own kernels, straight from ``.weight``; a table that is called as a module takes
+``functional.embedding_rows`` on a HIP device.
+
+``LayerNorm``, ``Linear`` and ``GatedLinear`` are the layers of a deeper ranking head
+(``collie_amd.functional``) with the parameter names and the initialisation of their ``torch.nn``
+counterparts.
 """
-from typing import Dict, List
+from typing import Dict, List, Optional
 
 import torch
 
+from collie_amd import _lib, functional
 
-class ScaledEmbedding(torch.nn.Embedding):
+
+class _Table(torch.nn.Embedding):
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        # what the kernels do not take (other devices and types, renormalised rows, gradients
+        # divided by counts) stays torch's
+        if (not self.weight.is_cuda or self.weight.dtype not in _lib.ELEMENT_TYPES
+                or not input.is_cuda or input.dtype not in (torch.int32, torch.int64)
+                or self.max_norm is not None or self.scale_grad_by_freq):
+            return super().forward(input)
+        return functional.embedding_rows(self.weight, input, padding_idx=self.padding_idx,
+                                         sparse=self.sparse)
+
+
+class ScaledEmbedding(_Table):
     """N(0, (1 / (2.5 * embedding_dim))^2) initialisation (``layers.py:6-10``)."""
 
     def reset_parameters(self) -> None:
         self.weight.data.normal_(0, 1.0 / (self.embedding_dim * 2.5))
 
 
-class ZeroEmbedding(torch.nn.Embedding):
+class ZeroEmbedding(_Table):
     """All-zero initialisation (``layers.py:13-17``)."""
 
     def reset_parameters(self) -> None:
         self.weight.data.zero_()
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """``torch.nn.LayerNorm`` over the last dimension (``functional.layer_norm``)."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-5, elementwise_affine: bool = True,
+                 bias: bool = True, device=None, dtype=None):
+        if not isinstance(normalized_shape, int):
+            raise ValueError('LayerNorm normalises the last dimension only: expected an int, not '
+                             f'{normalized_shape!r}')
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device, dtype)
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if input.shape[-1:] != self.normalized_shape:
+            raise ValueError(f'expected [..., {self.normalized_shape[0]}], not {tuple(input.shape)}')
+        return functional.layer_norm(input, self.weight, self.bias, self.eps)
+
+
+class Linear(torch.nn.Linear):
+    """``torch.nn.Linear`` with an activation and an optional residual that is added to its result
+    (``functional.linear``)."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 activation: str = 'identity', device=None, dtype=None):
+        if activation not in _lib.ACTIVATIONS:
+            raise ValueError(f'{activation!r} is not an activation: {", ".join(_lib.ACTIVATIONS)}')
+        super().__init__(in_features, out_features, bias, device, dtype)
+        self.activation = activation
+
+    def forward(self, input: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return functional.linear(input, self.weight, self.bias, self.activation, residual)
+
+
+class GatedLinear(torch.nn.Module):
+    """``activation(gate(x)) * up(x)`` with two ``torch.nn.Linear`` parameter sets ``gate`` and
+    ``up`` (``functional.gated_linear``)."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 activation: str = 'silu', device=None, dtype=None):
+        if activation not in _lib.ACTIVATIONS:
+            raise ValueError(f'{activation!r} is not an activation: {", ".join(_lib.ACTIVATIONS)}')
+        super().__init__()
+        self.gate = torch.nn.Linear(in_features, out_features, bias, device, dtype)
+        self.up = torch.nn.Linear(in_features, out_features, bias, device, dtype)
+        self.activation = activation
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        return functional.gated_linear(input, self.gate.weight, self.up.weight, self.gate.bias,
+                                       self.up.bias, self.activation)
 
 
 class MultiOptimizer(object):

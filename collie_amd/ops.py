@@ -2,6 +2,7 @@
 Thin tensor-level wrappers over the C ABI: they only marshal torch tensors (device pointers,
 current HIP stream) into ``libcollie_hip.so`` calls.  No arithmetic happens in this file.
 """
+import contextlib
 import ctypes
 from ctypes import byref, c_void_p
 
@@ -927,3 +928,257 @@ def eval_merge_topk(cand_scores, cand_ids, k):
                                            ptr(scores),
                                            ptr(ids), stream_ptr()), 'collie_mf_eval_merge_topk')
     return scores, ids
+
+
+# ---- layers of a deeper ranking head ---------------------------------------------------------------
+_ON_CURRENT = contextlib.nullcontext()
+
+
+def _on_device(t):
+    """Context in which ``t``'s device is the current one (whose stream the launches take)."""
+    if t.device.index == torch.cuda.current_device():
+        return _ON_CURRENT
+    return torch.cuda.device(t.device)
+
+
+def element_type(t, what):
+    tag = _lib.ELEMENT_TYPES.get(t.dtype)
+    if tag is None:
+        raise _lib.CollieHipError(f'{what} must be float32, bfloat16 or float16, not {t.dtype}')
+    return tag
+
+
+def rows_view(t, width):
+    """``t`` as [rows, width] with contiguous rows that do not overlap (a copy only if it must be),
+    and the distance of its rows in elements."""
+    if not t.is_contiguous():
+        if t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+            t = t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    return t, (t.stride(0) if t.shape[0] > 1 else width)
+
+
+def embedding_rows(table, ids, scale=1.0, status=None):
+    """``scale * table[ids]`` (``collie_embedding_rows``): [*ids.shape, dim]."""
+    require_hip(table, 'table')
+    require_hip(ids, 'ids')
+    tag = element_type(table, 'table')
+    if table.dim() != 2:
+        raise ValueError(f'table must be [rows, dim], not {tuple(table.shape)}')
+    if ids.device != table.device:
+        raise _lib.CollieHipError(f'ids are on {ids.device}, the table is on {table.device}')
+    table, ids = table.contiguous(), ids.contiguous()
+    out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
+    with _on_device(table):
+        check(load().collie_embedding_rows(
+            ptr(table), tag, table.shape[0], table.shape[1], ptr(ids), idx_dtype(ids), ids.numel(),
+            float(scale), ptr(out), ptr(status), stream_ptr()), 'collie_embedding_rows')
+    return out
+
+
+def embedding_rows_grad(ids, dy, num_rows, scale=1.0, padding_idx=None, status=None):
+    """Gradient of ``embedding_rows`` with respect to the table, [num_rows, dim] in ``dy``'s type,
+    summed in the order of ``ids`` (``collie_embedding_rows_grad``)."""
+    require_hip(dy, 'dy')
+    require_hip(ids, 'ids')
+    tag = element_type(dy, 'dy')
+    dim = dy.shape[-1]
+    if dy.shape[:-1] != ids.shape:
+        raise ValueError(f'dy {tuple(dy.shape)} does not belong to ids {tuple(ids.shape)}')
+    if ids.device != dy.device:
+        raise _lib.CollieHipError(f'ids are on {ids.device}, dy is on {dy.device}')
+    n = ids.numel()
+    ids = ids.contiguous()
+    dy, ld = rows_view(dy, dim)
+    grad = torch.empty(num_rows, dim, dtype=dy.dtype, device=dy.device)
+    need = int(load().collie_embedding_rows_grad_workspace_bytes(n, dim))
+    workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    with _on_device(dy):
+        check(load().collie_embedding_rows_grad(
+            ptr(ids), idx_dtype(ids), n, ptr(dy), ld, tag, num_rows, dim, float(scale),
+            -1 if padding_idx is None else int(padding_idx), ptr(grad), ptr(workspace), need,
+            ptr(status), stream_ptr()), 'collie_embedding_rows_grad')
+    return grad
+
+
+def _param(t, like, shape, what, other=None):
+    """A parameter of a layer: on ``like``'s device, of its type (or ``other``'s), contiguous."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise ValueError(f'{what} must have shape {shape}, not {tuple(t.shape)}')
+    if t.device != like.device:
+        raise _lib.CollieHipError(f'{what} is on {t.device}, x is on {like.device}')
+    if t.dtype != like.dtype and t.dtype != other:
+        raise _lib.CollieHipError(f'{what} is {t.dtype}, x is {like.dtype}')
+    return t.contiguous()
+
+
+def _norm_params(x, weight, bias):
+    dim = x.shape[-1]
+    weight = _param(weight, x, (dim,), 'weight', torch.float32)
+    bias = _param(bias, x, (dim,), 'bias', torch.float32)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise _lib.CollieHipError(f'weight is {weight.dtype}, bias is {bias.dtype}')
+    given = weight if weight is not None else bias
+    return weight, bias, element_type(given if given is not None else x, 'weight')
+
+
+def layer_norm_forward(x, weight, bias, eps, keep):
+    """(y, mean, rstd) of ``collie_layer_norm_forward``; mean and rstd (per row, float32) only with
+    ``keep``."""
+    require_hip(x, 'x')
+    tag = element_type(x, 'x')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f'x must have a last dimension to normalise, not {tuple(x.shape)}')
+    dim = x.shape[-1]
+    weight, bias, w_tag = _norm_params(x, weight, bias)
+    rows, ld = rows_view(x, dim)
+    m = rows.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if keep:
+        mean = torch.empty(m, dtype=torch.float32, device=x.device)
+        rstd = torch.empty(m, dtype=torch.float32, device=x.device)
+    with _on_device(x):
+        check(load().collie_layer_norm_forward(
+            ptr(rows), ld, tag, m, dim, ptr(weight), ptr(bias), w_tag, float(eps), ptr(y),
+            ptr(mean), ptr(rstd), stream_ptr()), 'collie_layer_norm_forward')
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, weight, bias, mean, rstd, want):
+    """(dx, dweight, dbias) of ``collie_layer_norm_backward``, each None unless ``want`` says so."""
+    dim = x.shape[-1]
+    weight, bias, w_tag = _norm_params(x, weight, bias)
+    rows, ld = rows_view(x, dim)
+    g, g_ld = rows_view(dy, dim)
+    m = rows.shape[0]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
+    dw = torch.empty_like(weight) if want[1] and weight is not None else None
+    db = torch.empty_like(bias) if want[2] and bias is not None else None
+    need = int(load().collie_layer_norm_backward_workspace_bytes(m, dim))
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    with _on_device(x):
+        check(load().collie_layer_norm_backward(
+            ptr(g), g_ld, ptr(rows), ld, element_type(x, 'x'), m, dim, ptr(weight), w_tag, ptr(mean),
+            ptr(rstd), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need, stream_ptr()),
+            'collie_layer_norm_backward')
+    return dx, dw, db
+
+
+def activation_code(name):
+    code = _lib.ACTIVATIONS.get(name)
+    if code is None:
+        raise ValueError(f'{name!r} is not an activation: {", ".join(_lib.ACTIVATIONS)}')
+    return code
+
+
+def _layer_args(x, weight, biases, second=None):
+    """Checked (rows of x, their distance, weights, biases, m, n_in, n_out) of a layer."""
+    require_hip(x, 'x')
+    element_type(x, 'x')
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit: expected '
+                         'x [..., n_in] and weight [n_out, n_in]')
+    n_out, n_in = weight.shape
+    if n_out < 1 or n_in < 1:
+        raise ValueError(f'weight {tuple(weight.shape)} is empty')
+    weights = [_param(weight, x, (n_out, n_in), 'weight')]
+    if second is not None:
+        weights.append(_param(second, x, (n_out, n_in), 'weight'))
+    biases = [_param(b, x, (n_out,), 'bias') for b in biases]
+    rows, ld = rows_view(x, n_in)
+    return rows, ld, weights, biases, rows.shape[0], n_in, n_out
+
+
+def linear_forward(x, weight, bias, activation, residual, keep):
+    """(y, kept pre-activations or None) of ``collie_linear_forward``."""
+    act = activation_code(activation)
+    rows, ld, (weight,), (bias,), m, n_in, n_out = _layer_args(x, weight, (bias,))
+    shape = (*x.shape[:-1], n_out)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    res, res_ld = None, 0
+    if residual is not None:
+        res = _param_rows(residual, x, shape, 'residual')
+        res, res_ld = rows_view(res, n_out)
+    kept = torch.empty(m, n_out, dtype=x.dtype, device=x.device) if keep and act else None
+    with _on_device(x):
+        check(load().collie_linear_forward(
+            ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(weight), ptr(bias), n_out, act,
+            ptr(res), res_ld, ptr(kept), ptr(y), stream_ptr()), 'collie_linear_forward')
+    return y, kept
+
+
+def _param_rows(t, like, shape, what):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what} must have shape {tuple(shape)}, not {tuple(t.shape)}')
+    if t.device != like.device or t.dtype != like.dtype:
+        raise _lib.CollieHipError(f'{what} is {t.dtype} on {t.device}, x is {like.dtype} on '
+                                  f'{like.device}')
+    return t
+
+
+def _layer_workspace(x, m, n_in, n_out, pair):
+    need = int(load().collie_layer_backward_workspace_bytes(element_type(x, 'x'), m, n_in, n_out,
+                                                            pair))
+    return torch.empty(need, dtype=torch.uint8, device=x.device), need
+
+
+def linear_backward(dy, x, weight, activation, kept, want):
+    """(dx, dweight, dbias) of ``collie_linear_backward``, each None unless ``want`` says so."""
+    act = activation_code(activation)
+    rows, ld, (weight,), _, m, n_in, n_out = _layer_args(x, weight, ())
+    if m == 0:
+        return tuple(torch.zeros(s, dtype=x.dtype, device=x.device) if w else None for w, s in
+                     zip(want, (x.shape, weight.shape, (n_out,))))
+    g, g_ld = rows_view(dy, n_out)
+    dx, dw, db = (torch.empty(s, dtype=x.dtype, device=x.device) if w else None for w, s in
+                  zip(want, (x.shape, weight.shape, (n_out,))))
+    workspace, need = _layer_workspace(x, m, n_in, n_out, 0)
+    with _on_device(x):
+        check(load().collie_linear_backward(
+            ptr(g), g_ld, ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(weight), n_out, act,
+            ptr(kept), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need, stream_ptr()),
+            'collie_linear_backward')
+    return dx, dw, db
+
+
+def gated_forward(x, gate_weight, up_weight, gate_bias, up_bias, activation, keep):
+    """(y, kept gate, kept up) of ``collie_gated_forward``; the kept ones None without ``keep``."""
+    act = activation_code(activation)
+    if (gate_bias is None) != (up_bias is None):
+        raise ValueError('gate_bias and up_bias: both or none')
+    rows, ld, (wg, wu), (bg, bu), m, n_in, n_out = _layer_args(x, gate_weight,
+                                                               (gate_bias, up_bias), up_weight)
+    y = torch.empty(*x.shape[:-1], n_out, dtype=x.dtype, device=x.device)
+    g = u = None
+    if keep:
+        g = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
+        u = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
+    with _on_device(x):
+        check(load().collie_gated_forward(
+            ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(wg), ptr(wu), ptr(bg), ptr(bu), n_out,
+            act, ptr(g), ptr(u), ptr(y), stream_ptr()), 'collie_gated_forward')
+    return y, g, u
+
+
+def gated_backward(dy, x, gate_weight, up_weight, activation, kept_gate, kept_up, want):
+    """(dx, dgate_weight, dup_weight, dgate_bias, dup_bias) of ``collie_gated_backward``, each None
+    unless ``want`` says so."""
+    act = activation_code(activation)
+    rows, ld, (wg, wu), _, m, n_in, n_out = _layer_args(x, gate_weight, (), up_weight)
+    shapes = (x.shape, wg.shape, wu.shape, (n_out,), (n_out,))
+    make = torch.zeros if m == 0 else torch.empty
+    out = [make(s, dtype=x.dtype, device=x.device) if w else None for w, s in zip(want, shapes)]
+    if m == 0:
+        return tuple(out)
+    dy, dy_ld = rows_view(dy, n_out)
+    workspace, need = _layer_workspace(x, m, n_in, n_out, 1)
+    with _on_device(x):
+        check(load().collie_gated_backward(
+            ptr(dy), dy_ld, ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(wg), ptr(wu), n_out,
+            act, ptr(kept_gate), ptr(kept_up), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]),
+            ptr(out[4]), ptr(workspace), need, stream_ptr()), 'collie_gated_backward')
+    return tuple(out)

@@ -36,6 +36,9 @@ typedef void* collie_stream_t; /* hipStream_t */
 
 enum { COLLIE_I32 = 0, COLLIE_I64 = 1 };
 
+/* element types of the ranking-head operators (embedding rows, layer norm, linear, gated layer) */
+enum { COLLIE_F32 = 0, COLLIE_BF16 = 1, COLLIE_F16 = 2 };
+
 /* collie/loss/{bpr,hinge,warp}.py of the reference; the adaptive variants are what base_pipeline.py:307-338 selects
  * whenever num_negative_samples > 1 */
 enum {
@@ -800,6 +803,85 @@ int collie_dense_rows_update(float* table, int64_t num_rows, int32_t dim, const 
                              const collie_optim_cfg* cfg, float* state1, float* state2,
                              int32_t* row_stamp, void* workspace, size_t workspace_bytes,
                              int32_t* status, collie_stream_t stream);
+
+/* ---- layers of a deeper ranking head -----------------------------------------------------------
+ * Embedding rows with scaling, layer normalisation, the linear layer with bias, activation and
+ * residual, and the gated layer, each with its gradient.  Values are float32, bfloat16 or float16
+ * (COLLIE_F32 / COLLIE_BF16 / COLLIE_F16), sums and statistics float32; a result is rounded once.
+ * Rows may be apart by more than their width (`*_ld`, in elements, >= the width); tables, weights,
+ * biases, kept values and results are contiguous.  No entry point uses floating-point atomics: equal
+ * calls give equal bits.  Workspaces hold nothing between calls. */
+
+/* y[i] = scale * table[ids[i]] ([n, dim]); an id outside [0, num_rows) gives a zero row and sets bit
+ * 0 of *status.  What nn.Embedding.forward computes (collie/model/base/layers.py:6-17) at scale 1. */
+int collie_embedding_rows(const void* table, int32_t dtype, int64_t num_rows, int32_t dim,
+                          const void* ids, int32_t ids_dtype, int64_t n, float scale, void* out,
+                          int32_t* status, collie_stream_t stream);
+
+/* grad[r] = scale * sum of dy[i] over ids[i] = r, every row of [num_rows, dim] written (0 without an
+ * entry); ids outside the table and `padding_idx` (-1: none) take no gradient.  grad: 16-byte
+ * aligned; workspace: collie_embedding_rows_grad_workspace_bytes(n, dim); n < 2^30. */
+size_t collie_embedding_rows_grad_workspace_bytes(int64_t n, int32_t dim);
+int collie_embedding_rows_grad(const void* ids, int32_t ids_dtype, int64_t n, const void* dy,
+                               int64_t dy_ld, int32_t dtype, int64_t num_rows, int32_t dim,
+                               float scale, int64_t padding_idx, void* grad, void* workspace,
+                               size_t workspace_bytes, int32_t* status, collie_stream_t stream);
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (biased variance).
+ * weight / bias (NULL: ones / zeros) are float32 or of x's type (w_dtype); mean / rstd [rows] are
+ * written for the backward pass (NULL: not wanted). */
+int collie_layer_norm_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t rows, int32_t dim,
+                              const void* weight, const void* bias, int32_t w_dtype, float eps,
+                              void* y, float* mean, float* rstd, collie_stream_t stream);
+
+/* dx (NULL: not wanted), and dweight / dbias of w_dtype (NULL: not wanted), summed over the rows;
+ * rows = 0 gives zeros. */
+size_t collie_layer_norm_backward_workspace_bytes(int64_t rows, int32_t dim);
+int collie_layer_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld,
+                               int32_t dtype, int64_t rows, int32_t dim, const void* weight,
+                               int32_t w_dtype, const float* mean, const float* rstd, void* dx,
+                               void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                               collie_stream_t stream);
+
+enum {
+  COLLIE_ACT_IDENTITY = 0,
+  COLLIE_ACT_RELU = 1,
+  COLLIE_ACT_LEAKY_RELU = 2, /* slope 0.01, as in the hybrid head */
+  COLLIE_ACT_SIGMOID = 3,
+  COLLIE_ACT_SILU = 4,       /* z sigmoid(z) */
+  COLLIE_ACT_GELU = 5        /* z Phi(z), with erf */
+};
+
+/* y = act(x weight^T + bias) + residual ([m, n_out]); weight [n_out, n_in]; bias / residual may be
+ * NULL.  keep [m, n_out] (NULL: not wanted) takes the pre-activations, in x's type (float16:
+ * finite ones beyond +-65504 as that), for the backward pass. */
+int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
+                          const void* weight, const void* bias, int32_t n_out, int32_t act,
+                          const void* residual, int64_t res_ld, void* keep, void* y,
+                          collie_stream_t stream);
+
+/* y = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias); both biases or none; keep_gate /
+ * keep_up as above. */
+int collie_gated_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
+                         const void* gate_weight, const void* up_weight, const void* gate_bias,
+                         const void* up_bias, int32_t n_out, int32_t act, void* keep_gate,
+                         void* keep_up, void* y, collie_stream_t stream);
+
+/* Gradients from dy [m, n_out] (that of the residual is dy itself), m >= 1; every output may be NULL
+ * (not wanted).  kept_z is NULL for the identity.  workspace:
+ * collie_layer_backward_workspace_bytes(dtype, m, n_in, n_out, pair = 0 linear / 1 gated). */
+size_t collie_layer_backward_workspace_bytes(int32_t dtype, int64_t m, int32_t n_in, int32_t n_out,
+                                             int32_t pair);
+int collie_linear_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int32_t dtype,
+                           int64_t m, int32_t n_in, const void* weight, int32_t n_out, int32_t act,
+                           const void* kept_z, void* dx, void* dweight, void* dbias, void* workspace,
+                           size_t workspace_bytes, collie_stream_t stream);
+int collie_gated_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int32_t dtype,
+                          int64_t m, int32_t n_in, const void* gate_weight, const void* up_weight,
+                          int32_t n_out, int32_t act, const void* kept_gate, const void* kept_up,
+                          void* dx, void* dgate_weight, void* dup_weight, void* dgate_bias,
+                          void* dup_bias, void* workspace, size_t workspace_bytes,
+                          collie_stream_t stream);
 
 #ifdef __cplusplus
 }
