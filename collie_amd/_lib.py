@@ -250,14 +250,17 @@ SIGNATURES = {
                                                   c_int64, c_int32, c_void_p, c_int32, c_void_p,
                                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                   c_size_t, c_void_p]),
+    'collie_layer_forward_workspace_bytes': (c_size_t, [c_void_p, c_int64, c_int32, c_int64, c_int32,
+                                                        c_void_p, c_void_p, c_int32]),
+    'collie_layer_backward_workspace_bytes': (c_size_t, [c_void_p, c_int64, c_void_p, c_int64,
+                                                         c_int32, c_int64, c_int32, c_void_p,
+                                                         c_void_p, c_int32, c_int32]),
     'collie_linear_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
                                              c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
-                                             c_void_p, c_void_p]),
+                                             c_void_p, c_void_p, c_size_t, c_void_p]),
     'collie_gated_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
                                             c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
-                                            c_void_p, c_void_p, c_void_p]),
-    'collie_layer_backward_workspace_bytes': (c_size_t, [c_int32, c_int64, c_int32, c_int32,
-                                                         c_int32]),
+                                            c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     'collie_linear_backward': (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64,
                                               c_int32, c_void_p, c_int32, c_int32, c_void_p,
                                               c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,

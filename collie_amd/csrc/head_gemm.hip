@@ -8,154 +8,12 @@
 // the gated forward pass has two accumulators per output, the gated dx runs over [dg | du] and
 // [Wg ; Wu] as one product of twice the depth, and both weight gradients are one product whose rows
 // are the columns of [dg | du].  Products are summed in float32.
-#include "head_act.h"
+#include "head_tile.h"
 
 namespace collie {
 namespace {
 
 constexpr int kBlock = 256;
-
-// element (i, k) of an operand: p[i * rs + k * ks]
-struct Mat {
-  const void* p;
-  int64_t rs, ks;
-};
-
-enum Epilogue { kEpiLinear, kEpiGated, kEpiStore, kEpiPartial };
-
-struct Gemm {
-  Mat a, b;
-  const void* b2;        // second matrix of b's shape, or NULL
-  int64_t k_split;       // without kEpiGated: k >= k_split reads b2 at k - k_split, and of either
-  int64_t k_valid;       // matrix only the first k_valid are there (the rest is padding: zero)
-  int64_t m, n, k;
-  int64_t k_chunk;       // depth of one of the `splits` parts
-  int splits;
-  // epilogue
-  int act;
-  const void *bias, *bias2;
-  const void* residual;
-  int64_t res_ld;
-  void *keep, *keep2;    // pre-activations for the backward pass [m, n], or NULL
-  void *c, *c2;          // output [m, n]; with kEpiStore rows >= row_split are c2's, and of either
-  int64_t row_split;     // only the first row_valid are wanted
-  int64_t row_valid;
-  float* partial;        // kEpiPartial: [splits, m, n]
-};
-
-// results at (row, col .. col + W): columns of one row that one thread holds
-template <typename T, int EPI, int W>
-__device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t col, float (&v)[W],
-                                           float (&u)[W]) {
-  if (row >= g.m || col >= g.n) return;
-  const int left = g.n - col < W ? static_cast<int>(g.n - col) : W;
-  const int64_t at = row * g.n + col;
-  if constexpr (EPI == kEpiPartial) {
-    store_pack<float, W>(g.partial + static_cast<int64_t>(blockIdx.z) * g.m * g.n + at, left, v);
-  } else if constexpr (EPI == kEpiStore) {
-    T* c = static_cast<T*>(row < g.row_split ? g.c : g.c2);
-    const int64_t r = row < g.row_split ? row : row - g.row_split;
-    if (c && r < g.row_valid) store_pack<T, W>(c + r * g.n + col, left, v);
-  } else {
-    float add[W];
-    if (g.bias) {
-      load_pack<T, W>(static_cast<const T*>(g.bias) + col, left, add);
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += add[j];
-      if constexpr (EPI == kEpiGated) {
-        load_pack<T, W>(static_cast<const T*>(g.bias2) + col, left, add);
-#pragma unroll
-        for (int j = 0; j < W; ++j) u[j] += add[j];
-      }
-    }
-    if (g.keep) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) add[j] = kept<T>(v[j]);
-      store_pack<T, W>(static_cast<T*>(g.keep) + at, left, add);
-      if constexpr (EPI == kEpiGated) {
-#pragma unroll
-        for (int j = 0; j < W; ++j) add[j] = kept<T>(u[j]);
-        store_pack<T, W>(static_cast<T*>(g.keep2) + at, left, add);
-      }
-    }
-    act_values(g.act, v);
-    if constexpr (EPI == kEpiGated) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[j] *= u[j];
-    } else if (g.residual) {
-      load_pack<T, W>(static_cast<const T*>(g.residual) + row * g.res_ld + col, left, add);
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += add[j];
-    }
-    store_pack<T, W>(static_cast<T*>(g.c) + at, left, v);
-  }
-}
-
-// ---- any sizes, any strides: 64 x 64 results per workgroup, 4 x 4 per thread ----------------------
-constexpr int kTile = 64, kDepth = 16;
-
-template <typename T, int EPI>
-__global__ __launch_bounds__(kBlock) void gemm_any_kernel(const Gemm g) {
-  constexpr bool PAIR = EPI == kEpiGated;
-  __shared__ float as[kDepth][kTile + 4], bs[kDepth][kTile + 4], us[PAIR ? kDepth : 1][kTile + 4];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int64_t col0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const int64_t k0 = static_cast<int64_t>(blockIdx.z) * g.k_chunk;
-  const int64_t k1 = k0 + g.k_chunk < g.k ? k0 + g.k_chunk : g.k;
-  float acc[4][4], acc2[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = acc2[i][j] = 0.0f;
-  for (int64_t kk = k0; kk < k1; kk += kDepth) {
-    for (int e = threadIdx.x; e < kTile * kDepth; e += kBlock) {
-      // neighbouring threads walk the direction that is contiguous in memory
-      const int ak = g.a.ks == 1 ? e % kDepth : e / kTile, ai = g.a.ks == 1 ? e / kDepth : e % kTile;
-      const int64_t r = row0 + ai, k = kk + ak;
-      as[ak][ai] = r < g.m && k < k1 ? static_cast<float>(static_cast<const T*>(
-                                           g.a.p)[r * g.a.rs + k * g.a.ks]) : 0.0f;
-      const int bk = g.b.ks == 1 ? e % kDepth : e / kTile, bi = g.b.ks == 1 ? e / kDepth : e % kTile;
-      const int64_t c = col0 + bi;
-      int64_t kb = kk + bk;
-      bool in = c < g.n && kb < k1;
-      const T* b = static_cast<const T*>(g.b.p);
-      if (PAIR) {
-        us[PAIR ? bk : 0][bi] = in ? static_cast<float>(static_cast<const T*>(
-                                         g.b2)[c * g.b.rs + kb * g.b.ks]) : 0.0f;
-      } else if (g.b2) {
-        if (kb >= g.k_split) {
-          b = static_cast<const T*>(g.b2);
-          kb -= g.k_split;
-        }
-        in = in && kb < g.k_valid;
-      }
-      bs[bk][bi] = in ? static_cast<float>(b[c * g.b.rs + kb * g.b.ks]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-      float a[4], b[4], u[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = as[k][ty * 4 + i];
-        b[i] = bs[k][tx * 4 + i];
-        if (PAIR) u[i] = us[PAIR ? k : 0][tx * 4 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-          if (PAIR) acc2[i][j] = fmaf(a[i], u[j], acc2[i][j]);
-        }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    finish_row<T, EPI, 4>(g, row0 + ty * 4 + i, col0 + tx * 4, acc[i], acc2[i]);
-}
 
 // ---- dz = dy f'(z) (linear), [dg | du] (gated), and the column sums for the bias gradients --------
 struct ActBwd {
@@ -231,11 +89,11 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
 }
 
 // out[c] = sum over `count` partials of partial[k][c], c < width, in fixed order; columns from
-// `split` on belong to out2, and of either only the first `valid` are wanted.  64 columns x 16 slices of the partials per workgroup.
+// `split` on belong to out2.  64 columns x 16 slices of the partials per workgroup.
 constexpr int kRedCols = 64, kRedRows = 16;
 template <typename T>
 __global__ __launch_bounds__(kRedCols* kRedRows) void sum_partials_kernel(
-    const float* __restrict__ partial, int64_t count, int64_t width, int64_t split, int64_t valid,
+    const float* __restrict__ partial, int64_t count, int64_t width, int64_t split,
     T* __restrict__ out, T* __restrict__ out2) {
   __shared__ float sh[kRedRows][kRedCols];
   const int cx = threadIdx.x % kRedCols, ry = threadIdx.x / kRedCols;
@@ -252,33 +110,145 @@ __global__ __launch_bounds__(kRedCols* kRedRows) void sum_partials_kernel(
 #pragma unroll
   for (int k = 0; k < kRedRows; ++k) t += sh[k][cx];
   T* o = c < split ? out : out2;
-  const int64_t at = c < split ? c : c - split;
-  if (o && at < valid) o[at] = static_cast<T>(t);
+  if (o) o[c < split ? c : c - split] = static_cast<T>(t);
 }
 
 template <typename T>
-int sum_partials(const float* partial, int64_t count, int64_t width, int64_t split, int64_t valid,
-                 void* out, void* out2, hipStream_t stream) {
+int sum_partials(const float* partial, int64_t count, int64_t width, int64_t split, void* out,
+                 void* out2, hipStream_t stream) {
   hipLaunchKernelGGL(sum_partials_kernel<T>, dim3(static_cast<unsigned>((width + kRedCols - 1) / kRedCols)),
                      dim3(kRedCols * kRedRows), 0, stream, partial, count, width, split,
-                     valid, static_cast<T*>(out), static_cast<T*>(out2));
+                     static_cast<T*>(out), static_cast<T*>(out2));
   return check_launch("sum_partials_kernel");
 }
 
-template <typename T, int EPI>
-int launch_gemm(const Gemm& g, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((g.m + kTile - 1) / kTile),
-                  static_cast<unsigned>((g.n + kTile - 1) / kTile), static_cast<unsigned>(g.splits));
-  hipLaunchKernelGGL((gemm_any_kernel<T, EPI>), grid, dim3(kBlock), 0, stream, g);
-  return check_launch("gemm_any_kernel");
+// ---- laying an operand out for the tiles -----------------------------------------------------------
+// The tiles load whole aligned 16-byte packs.  Rows of another width or alignment are copied once
+// into rows of whole packs, zeros behind them: one more pass over that operand, for odd widths only.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const T* __restrict__ src, int64_t ld,
+                                                           int64_t rows, int64_t cols, int64_t packs,
+                                                           T* __restrict__ dst) {
+  constexpr int V = kVec<T>;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlock;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < rows * packs;
+       i += stride) {
+    const int64_t row = i / packs, c = (i - row * packs) * V;
+    const int64_t left = cols - c;
+    float v[V];
+    load_pack<T, V>(src + row * ld + c, left < V ? static_cast<int>(left) : V, v);
+    store_pack<T, V>(dst + i * V, V, v);
+  }
 }
 
-// parts of the depth of a weight gradient: enough workgroups for every CU, each at least 256 deep
-int weight_splits(int64_t rows, int64_t n, int64_t m) {
-  const int64_t tiles = ((n + kTile - 1) / kTile) * ((m + kTile - 1) / kTile);
-  int64_t s = (1024 + tiles - 1) / tiles;
-  if (s > rows / 256) s = rows / 256;
-  return static_cast<int>(s < 1 ? 1 : s);
+template <typename T>
+bool whole_packs(const void* p, int64_t ld, int64_t cols) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % kVec<T> == 0 && cols % kVec<T> == 0;
+}
+
+// columns of a row of whole packs
+template <typename T>
+int64_t padded(int64_t n) {
+  return (n + kVec<T> - 1) / kVec<T> * kVec<T>;
+}
+
+// `p` laid out in rows of whole packs: itself, or its copy at `room`
+template <typename T>
+int lay_out(const void*& p, int64_t& ld, int64_t rows, int64_t cols, void* room, hipStream_t stream) {
+  if (whole_packs<T>(p, ld, cols)) return 0;
+  const int64_t packs = padded<T>(cols) / kVec<T>;
+  int64_t grid = (rows * packs + kBlock - 1) / kBlock;
+  if (grid > 8192) grid = 8192;
+  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(kBlock), 0, stream,
+                     static_cast<const T*>(p), ld, rows, cols, packs, static_cast<T*>(room));
+  p = room;
+  ld = padded<T>(cols);
+  return check_launch("pack_rows_kernel");
+}
+
+// ---- which kernel, and how many parts of the depth -------------------------------------------------
+constexpr int64_t kSkinnyRows = 64;  // rows of the kernel that streams the weights
+constexpr int64_t kCus = 256;
+
+struct Plan {
+  int tile;    // BM = BN
+  int splits;
+  int64_t k_chunk;
+};
+
+template <typename T>
+Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair) {
+  const int64_t depth = 128 / static_cast<int64_t>(sizeof(T));
+  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n * (pair ? 2 : 1) + t - 1) / t); };
+  Plan p;
+  // the large tile reads half as much from LDS per product, but one workgroup fills a CU
+  p.tile = sizeof(T) == 2 && tiles(256) >= kCus ? 256 : 128;
+  // too few tiles for the chip: the depth is cut until there are about two workgroups per CU, in
+  // parts of at least four stages
+  int64_t s = (2 * kCus) / tiles(p.tile);
+  if (s > k / (4 * depth)) s = k / (4 * depth);
+  if (s < 1) s = 1;
+  p.k_chunk = ((k + s - 1) / s + depth - 1) / depth * depth;
+  p.splits = static_cast<int>((k + p.k_chunk - 1) / p.k_chunk);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+template <typename T>
+size_t partial_floats(int64_t m, int64_t n, int64_t k, bool pair) {
+  const Plan p = plan_gemm<T>(m, n, k, pair);
+  return p.splits > 1 ? static_cast<size_t>(p.splits) * (pair ? 2 : 1) * m * n : 0;
+}
+
+template <typename T, bool AKC, bool BKC, int EPI, bool CAT>
+int launch_tiles(Gemm& g, hipStream_t stream) {
+  constexpr bool PAIR = EPI == kEpiGated;
+  const Plan p = plan_gemm<T>(g.m, g.n, g.k, PAIR);
+  g.splits = p.splits;
+  g.k_chunk = p.k_chunk;
+  g.b2_offset = g.b2 ? (reinterpret_cast<intptr_t>(g.b2) - reinterpret_cast<intptr_t>(g.b.p)) /
+                           static_cast<intptr_t>(sizeof(T))
+                     : 0;
+  const int64_t tn = PAIR ? p.tile / 2 : p.tile;
+  const int64_t total = ((g.m + p.tile - 1) / p.tile) * ((g.n + tn - 1) / tn) * p.splits;
+  COLLIE_REQUIRE(total < (int64_t{1} << 31), "matrix product: too many tiles");
+  const dim3 grid(static_cast<unsigned>(total));
+  if (p.tile == 256) {
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, CAT>), grid, dim3(512),
+                         0, stream, g);
+  } else {
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, CAT>), grid, dim3(256), 0,
+                       stream, g);
+  }
+  if (check_launch("gemm_tile_kernel")) return -2;
+  if (p.splits == 1) return 0;
+  const int64_t blocks = (g.m * ((g.n + 3) / 4) + kWave - 1) / kWave;
+  if (p.splits <= 8)
+    hipLaunchKernelGGL((gemm_finish_kernel<T, EPI, 1>), dim3(static_cast<unsigned>(blocks)),
+                       dim3(kWave), 0, stream, g);
+  else
+    hipLaunchKernelGGL((gemm_finish_kernel<T, EPI, 8>), dim3(static_cast<unsigned>(blocks)),
+                       dim3(kWave * 8), 0, stream, g);
+  return check_launch("gemm_finish_kernel");
+}
+
+template <typename T, int EPI>
+int launch_skinny(const Gemm& g, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((g.n + 15) / 16)), block(kWave * kSkinnyWaves);
+  const bool whole = g.k % kVec<T> == 0;
+#define COLLIE_SKINNY(MT)                                                                        \
+  if (g.m <= 16 * MT) {                                                                          \
+    auto* kernel = whole ? gemm_skinny_kernel<T, MT, EPI, true> : gemm_skinny_kernel<T, MT, EPI, false>; \
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);                                       \
+    return check_launch("gemm_skinny_kernel");                                                   \
+  }
+  COLLIE_SKINNY(1)
+  COLLIE_SKINNY(2)
+  COLLIE_SKINNY(4)
+#undef COLLIE_SKINNY
+  set_error("matrix product: too many rows for the streaming kernel");
+  return -1;
 }
 
 // rows per slice of the column sums, and slices
@@ -288,30 +258,57 @@ int64_t act_parts(int64_t m) {
   return parts < kActParts ? parts : kActParts;
 }
 
-// columns of one half of dz: whole 16-byte packs
-int64_t padded(int64_t n, int32_t dtype) {
-  const int64_t v = 16 / static_cast<int64_t>(type_size(dtype));
-  return (n + v - 1) / v * v;
-}
-
-struct BwdWs {
-  void* dz;
-  float* act_partial;
-  float* w_partial;
-  int splits;
+// Workspaces.  An operand's room is there only if the operand is not in whole packs already.
+struct FwdWs {
+  void *x, *w, *w2;
+  float* partial;
   size_t bytes;
 };
 
-BwdWs carve_bwd(void* base, int32_t dtype, int64_t m, int64_t n_in, int64_t n_out, bool pair) {
+template <typename T>
+FwdWs carve_fwd(void* base, const void* x, int64_t x_ld, int64_t m, int64_t n_in, const void* w,
+                const void* w2, int64_t n_out) {
   Carver c(base);
-  BwdWs w;
-  const int64_t wide = pair ? 2 : 1;
-  w.dz = c.take<char>(static_cast<size_t>(m) * wide * padded(n_out, dtype) * type_size(dtype));
-  w.act_partial = c.take<float>(static_cast<size_t>(act_parts(m)) * wide * n_out);
-  w.splits = weight_splits(m, wide * n_out, n_in);
-  w.w_partial = c.take<float>(w.splits > 1 ? static_cast<size_t>(w.splits) * wide * padded(n_out, dtype) * n_in : 1);
-  w.bytes = align_up(c.off, 256);
-  return w;
+  FwdWs ws;
+  memset(&ws, 0, sizeof(ws));
+  if (m > kSkinnyRows) {
+    const size_t wide = static_cast<size_t>(padded<T>(n_in));
+    if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
+    if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
+    if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
+    ws.partial = c.take<float>(partial_floats<T>(m, n_out, n_in, w2 != nullptr));
+  }
+  ws.bytes = align_up(c.off, 256) + 256;
+  return ws;
+}
+
+struct BwdWs {
+  void *dz, *x, *w, *w2;
+  float* act_partial;
+  float* partial;
+  size_t bytes;
+};
+
+template <typename T>
+BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int64_t m,
+                int64_t n_in, const void* w, const void* w2, int64_t n_out, int act) {
+  Carver c(base);
+  BwdWs ws;
+  memset(&ws, 0, sizeof(ws));
+  const int64_t pair = w2 ? 2 : 1;
+  const int64_t half = padded<T>(n_out);
+  const size_t wide = static_cast<size_t>(padded<T>(n_in));
+  if (w2 || act != COLLIE_ACT_IDENTITY || !whole_packs<T>(dy, dy_ld, n_out))
+    ws.dz = c.take<T>(static_cast<size_t>(m) * pair * half);
+  if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
+  if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
+  if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
+  ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m)) * pair * n_out);
+  const size_t a = partial_floats<T>(m, n_in, (pair - 1) * half + n_out, false);
+  const size_t b = partial_floats<T>((pair - 1) * half + n_out, n_in, m, false);
+  ws.partial = c.take<float>(a > b ? a : b);
+  ws.bytes = align_up(c.off, 256) + 256;
+  return ws;
 }
 
 int check_layer(const char* who, int64_t m, int32_t n_in, int32_t n_out, int64_t x_ld, int32_t act) {
@@ -327,15 +324,13 @@ int check_layer(const char* who, int64_t m, int32_t n_in, int32_t n_out, int64_t
 template <typename T>
 int layer_forward(const void* x, int64_t x_ld, const void* w, const void* w2, const void* bias,
                   const void* bias2, const void* residual, int64_t res_ld, int64_t m, int64_t n_in,
-                  int64_t n_out, int act, void* keep, void* keep2, void* y, hipStream_t stream) {
+                  int64_t n_out, int act, void* keep, void* keep2, void* y, void* workspace,
+                  hipStream_t stream) {
   Gemm g;
   memset(&g, 0, sizeof(g));
-  g.a = {x, x_ld, 1};
-  g.b = {w, n_in, 1};
-  g.b2 = w2;
   g.m = m;
   g.n = n_out;
-  g.k = g.k_chunk = n_in;
+  g.k = n_in;
   g.splits = 1;
   g.act = act;
   g.bias = bias;
@@ -345,19 +340,34 @@ int layer_forward(const void* x, int64_t x_ld, const void* w, const void* w2, co
   g.keep = keep;
   g.keep2 = keep2;
   g.c = y;
-  return w2 ? launch_gemm<T, kEpiGated>(g, stream) : launch_gemm<T, kEpiLinear>(g, stream);
+  int64_t ld = n_in, ld2 = n_in;
+  if (m > kSkinnyRows) {
+    const FwdWs ws = carve_fwd<T>(workspace, x, x_ld, m, n_in, w, w2, n_out);
+    g.partial = ws.partial;
+    if (lay_out<T>(x, x_ld, m, n_in, ws.x, stream)) return -2;
+    if (lay_out<T>(w, ld, n_out, n_in, ws.w, stream)) return -2;
+    if (w2 && lay_out<T>(w2, ld2, n_out, n_in, ws.w2, stream)) return -2;
+  }
+  g.a = {x, x_ld, 1};
+  g.b = {w, ld, 1};
+  g.b2 = w2;
+  if (m <= kSkinnyRows)
+    return w2 ? launch_skinny<T, kEpiGated>(g, stream) : launch_skinny<T, kEpiLinear>(g, stream);
+  return w2 ? launch_tiles<T, true, true, kEpiGated, false>(g, stream)
+            : launch_tiles<T, true, true, kEpiLinear, false>(g, stream);
 }
 
 template <typename T>
 int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w,
-                   const void* w2, const void* z, const void* u, int32_t dtype, int64_t m,
-                   int64_t n_in, int64_t n_out, int act, void* dx, void* dw, void* dw2, void* db,
-                   void* db2, void* workspace, hipStream_t stream) {
+                   const void* w2, const void* z, const void* u, int64_t m, int64_t n_in,
+                   int64_t n_out, int act, void* dx, void* dw, void* dw2, void* db, void* db2,
+                   void* workspace, hipStream_t stream) {
   const bool pair = w2 != nullptr;
-  const BwdWs ws = carve_bwd(workspace, dtype, m, n_in, n_out, pair);
+  const BwdWs ws = carve_bwd<T>(workspace, dy, dy_ld, x, x_ld, m, n_in, w, w2, n_out, act);
   const int64_t wide = pair ? 2 : 1;
+  const int64_t half = padded<T>(n_out);
   const void* dz = dy;
-  int64_t dz_ld = dy_ld, half = n_out;
+  int64_t dz_ld = dy_ld;
   const bool sums = db || db2;
   if (z || sums) {
     ActBwd p;
@@ -370,10 +380,8 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     p.dy_ld = dy_ld;
     p.act = act;
     if (z) {
-      half = padded(n_out, dtype);
-      dz_ld = wide * half;
       dz = p.dz = ws.dz;
-      p.dz_ld = dz_ld;
+      dz_ld = p.dz_ld = wide * half;
     }
     p.partial = sums ? ws.act_partial : nullptr;
     const int64_t parts = act_parts(m);
@@ -386,45 +394,47 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
       hipLaunchKernelGGL((act_bwd_kernel<T, false>), grid, dim3(kBlock), 0, stream, p);
     if (check_launch("act_bwd_kernel")) return -2;
     if (sums) {
-      if (const int rc = sum_partials<T>(ws.act_partial, parts, wide * n_out, n_out, n_out, db, db2,
-                                           stream))
+      if (const int rc = sum_partials<T>(ws.act_partial, parts, wide * n_out, n_out, db, db2, stream))
         return rc;
     }
   }
+  if (!dx && !dw && !dw2) return 0;
+  if (!z && lay_out<T>(dz, dz_ld, m, n_out, ws.dz, stream)) return -2;
   Gemm g;
   if (dx) {
+    int64_t ld = n_in, ld2 = n_in;
+    if (lay_out<T>(w, ld, n_out, n_in, ws.w, stream)) return -2;
+    if (pair && lay_out<T>(w2, ld2, n_out, n_in, ws.w2, stream)) return -2;
     memset(&g, 0, sizeof(g));
     g.a = {dz, dz_ld, 1};
-    g.b = {w, 1, n_in};
+    g.b = {w, 1, ld};
     g.b2 = w2;
     g.k_split = half;
     g.k_valid = n_out;
     g.m = m;
     g.n = n_in;
-    g.k = g.k_chunk = pair ? half + n_out : n_out;
-    g.splits = 1;
+    g.k = pair ? half + n_out : n_out;
     g.c = dx;
     g.row_split = g.row_valid = m;
-    if (const int rc = launch_gemm<T, kEpiStore>(g, stream)) return rc;
+    g.partial = ws.partial;
+    const int rc = pair ? launch_tiles<T, true, false, kEpiStore, true>(g, stream)
+                        : launch_tiles<T, true, false, kEpiStore, false>(g, stream);
+    if (rc) return rc;
   }
   if (dw || dw2) {
+    if (lay_out<T>(x, x_ld, m, n_in, ws.x, stream)) return -2;
     memset(&g, 0, sizeof(g));
     g.a = {dz, 1, dz_ld};
     g.b = {x, 1, x_ld};
     g.m = pair ? half + n_out : n_out;
     g.n = n_in;
     g.k = m;
-    g.splits = ws.splits;
-    g.k_chunk = (m + g.splits - 1) / g.splits;
     g.row_split = half;
     g.row_valid = n_out;
     g.c = dw;
     g.c2 = dw2;
-    g.partial = ws.w_partial;
-    if (g.splits == 1) return launch_gemm<T, kEpiStore>(g, stream);
-    if (const int rc = launch_gemm<T, kEpiPartial>(g, stream)) return rc;
-    return sum_partials<T>(ws.w_partial, g.splits, g.m * g.n, half * g.n, n_out * g.n, dw, dw2,
-                           stream);
+    g.partial = ws.partial;
+    return launch_tiles<T, false, false, kEpiStore, false>(g, stream);
   }
   return 0;
 }
@@ -434,25 +444,52 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
 
 using namespace collie;
 
-extern "C" size_t collie_layer_backward_workspace_bytes(int32_t dtype, int64_t m, int32_t n_in,
-                                                        int32_t n_out, int32_t pair) {
+extern "C" size_t collie_layer_forward_workspace_bytes(const void* x, int64_t x_ld, int32_t dtype,
+                                                       int64_t m, int32_t n_in, const void* weight,
+                                                       const void* up_weight, int32_t n_out) {
   if (m < 1 || n_in < 1 || n_out < 1) return 256;
-  return carve_bwd(nullptr, dtype, m, n_in, n_out, pair != 0).bytes;
+  size_t bytes = 0;
+  with_type(dtype, "layer_forward", [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    bytes = carve_fwd<T>(nullptr, x, x_ld, m, n_in, weight, up_weight, n_out).bytes;
+    return 0;
+  });
+  return bytes;
+}
+
+extern "C" size_t collie_layer_backward_workspace_bytes(const void* dy, int64_t dy_ld, const void* x,
+                                                        int64_t x_ld, int32_t dtype, int64_t m,
+                                                        int32_t n_in, const void* weight,
+                                                        const void* up_weight, int32_t n_out,
+                                                        int32_t act) {
+  if (m < 1 || n_in < 1 || n_out < 1) return 256;
+  size_t bytes = 0;
+  with_type(dtype, "layer_backward", [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    bytes = carve_bwd<T>(nullptr, dy, dy_ld, x, x_ld, m, n_in, weight, up_weight, n_out, act).bytes;
+    return 0;
+  });
+  return bytes;
 }
 
 extern "C" int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m,
                                      int32_t n_in, const void* weight, const void* bias,
                                      int32_t n_out, int32_t act, const void* residual,
-                                     int64_t res_ld, void* keep, void* y, collie_stream_t stream_) {
+                                     int64_t res_ld, void* keep, void* y, void* workspace,
+                                     size_t workspace_bytes, collie_stream_t stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (check_layer("linear_forward", m, n_in, n_out, x_ld, act)) return -1;
   COLLIE_REQUIRE(!residual || m <= 1 || res_ld >= n_out, "linear_forward: rows of residual overlap");
   if (m == 0) return 0;
   COLLIE_REQUIRE(x && weight && y, "linear_forward: NULL pointer");
+  const size_t need =
+      collie_layer_forward_workspace_bytes(x, x_ld, dtype, m, n_in, weight, nullptr, n_out);
+  COLLIE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: need %zu bytes, got %zu",
+                 need, workspace_bytes);
   return with_type(dtype, "linear_forward", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     return layer_forward<T>(x, x_ld, weight, nullptr, bias, nullptr, residual, res_ld, m, n_in,
-                            n_out, act, keep, nullptr, y, stream);
+                            n_out, act, keep, nullptr, y, workspace, stream);
   });
 }
 
@@ -460,6 +497,7 @@ extern "C" int collie_gated_forward(const void* x, int64_t x_ld, int32_t dtype, 
                                     int32_t n_in, const void* gate_weight, const void* up_weight,
                                     const void* gate_bias, const void* up_bias, int32_t n_out,
                                     int32_t act, void* keep_gate, void* keep_up, void* y,
+                                    void* workspace, size_t workspace_bytes,
                                     collie_stream_t stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (check_layer("gated_forward", m, n_in, n_out, x_ld, act)) return -1;
@@ -469,10 +507,14 @@ extern "C" int collie_gated_forward(const void* x, int64_t x_ld, int32_t dtype, 
                  "gated_forward: keep_gate and keep_up belong together");
   if (m == 0) return 0;
   COLLIE_REQUIRE(x && gate_weight && up_weight && y, "gated_forward: NULL pointer");
+  const size_t need =
+      collie_layer_forward_workspace_bytes(x, x_ld, dtype, m, n_in, gate_weight, up_weight, n_out);
+  COLLIE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: need %zu bytes, got %zu",
+                 need, workspace_bytes);
   return with_type(dtype, "gated_forward", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     return layer_forward<T>(x, x_ld, gate_weight, up_weight, gate_bias, up_bias, nullptr, 0, m, n_in,
-                            n_out, act, keep_gate, keep_up, y, stream);
+                            n_out, act, keep_gate, keep_up, y, workspace, stream);
   });
 }
 
@@ -488,13 +530,14 @@ extern "C" int collie_linear_backward(const void* dy, int64_t dy_ld, const void*
   COLLIE_REQUIRE(dy && x && weight, "linear_backward: NULL pointer");
   COLLIE_REQUIRE((act == COLLIE_ACT_IDENTITY) == (kept_z == nullptr),
                  "linear_backward: kept_z is what the forward pass kept (NULL for the identity)");
-  const size_t need = collie_layer_backward_workspace_bytes(dtype, m, n_in, n_out, 0);
+  const size_t need = collie_layer_backward_workspace_bytes(dy, dy_ld, x, x_ld, dtype, m, n_in,
+                                                            weight, nullptr, n_out, act);
   COLLIE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: need %zu bytes, got %zu",
                  need, workspace_bytes);
   return with_type(dtype, "linear_backward", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    return layer_backward<T>(dy, dy_ld, x, x_ld, weight, nullptr, kept_z, nullptr, dtype, m, n_in,
-                             n_out, act, dx, dweight, nullptr, dbias, nullptr, workspace, stream);
+    return layer_backward<T>(dy, dy_ld, x, x_ld, weight, nullptr, kept_z, nullptr, m, n_in, n_out,
+                             act, dx, dweight, nullptr, dbias, nullptr, workspace, stream);
   });
 }
 
@@ -511,13 +554,14 @@ extern "C" int collie_gated_backward(const void* dy, int64_t dy_ld, const void* 
   COLLIE_REQUIRE(m >= 1, "gated_backward: no rows");
   COLLIE_REQUIRE(dy && x && gate_weight && up_weight && kept_gate && kept_up,
                  "gated_backward: NULL pointer");
-  const size_t need = collie_layer_backward_workspace_bytes(dtype, m, n_in, n_out, 1);
+  const size_t need = collie_layer_backward_workspace_bytes(
+      dy, dy_ld, x, x_ld, dtype, m, n_in, gate_weight, up_weight, n_out, act);
   COLLIE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: need %zu bytes, got %zu",
                  need, workspace_bytes);
   return with_type(dtype, "gated_backward", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    return layer_backward<T>(dy, dy_ld, x, x_ld, gate_weight, up_weight, kept_gate, kept_up, dtype, m,
-                             n_in, n_out, act, dx, dgate_weight, dup_weight, dgate_bias, dup_bias,
+    return layer_backward<T>(dy, dy_ld, x, x_ld, gate_weight, up_weight, kept_gate, kept_up, m, n_in,
+                             n_out, act, dx, dgate_weight, dup_weight, dgate_bias, dup_bias,
                              workspace, stream);
   });
 }

@@ -1104,10 +1104,13 @@ def linear_forward(x, weight, bias, activation, residual, keep):
         res = _param_rows(residual, x, shape, 'residual')
         res, res_ld = rows_view(res, n_out)
     kept = torch.empty(m, n_out, dtype=x.dtype, device=x.device) if keep and act else None
+    tag = element_type(x, 'x')
+    ws = _workspace(load().collie_layer_forward_workspace_bytes(
+        ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(None), n_out), x)
     with _on_device(x):
         check(load().collie_linear_forward(
-            ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(weight), ptr(bias), n_out, act,
-            ptr(res), res_ld, ptr(kept), ptr(y), stream_ptr()), 'collie_linear_forward')
+            ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(bias), n_out, act, ptr(res), res_ld,
+            ptr(kept), ptr(y), ptr(ws), ws.numel(), stream_ptr()), 'collie_linear_forward')
     return y, kept
 
 
@@ -1120,10 +1123,8 @@ def _param_rows(t, like, shape, what):
     return t
 
 
-def _layer_workspace(x, m, n_in, n_out, pair):
-    need = int(load().collie_layer_backward_workspace_bytes(element_type(x, 'x'), m, n_in, n_out,
-                                                            pair))
-    return torch.empty(need, dtype=torch.uint8, device=x.device), need
+def _workspace(need, like):
+    return torch.empty(int(need), dtype=torch.uint8, device=like.device)
 
 
 def linear_backward(dy, x, weight, activation, kept, want):
@@ -1136,12 +1137,13 @@ def linear_backward(dy, x, weight, activation, kept, want):
     g, g_ld = rows_view(dy, n_out)
     dx, dw, db = (torch.empty(s, dtype=x.dtype, device=x.device) if w else None for w, s in
                   zip(want, (x.shape, weight.shape, (n_out,))))
-    workspace, need = _layer_workspace(x, m, n_in, n_out, 0)
+    tag = element_type(x, 'x')
+    ws = _workspace(load().collie_layer_backward_workspace_bytes(
+        ptr(g), g_ld, ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(None), n_out, act), x)
     with _on_device(x):
         check(load().collie_linear_backward(
-            ptr(g), g_ld, ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(weight), n_out, act,
-            ptr(kept), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need, stream_ptr()),
-            'collie_linear_backward')
+            ptr(g), g_ld, ptr(rows), ld, tag, m, n_in, ptr(weight), n_out, act, ptr(kept), ptr(dx),
+            ptr(dw), ptr(db), ptr(ws), ws.numel(), stream_ptr()), 'collie_linear_backward')
     return dx, dw, db
 
 
@@ -1157,10 +1159,13 @@ def gated_forward(x, gate_weight, up_weight, gate_bias, up_bias, activation, kee
     if keep:
         g = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
         u = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
+    tag = element_type(x, 'x')
+    ws = _workspace(load().collie_layer_forward_workspace_bytes(
+        ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out), x)
     with _on_device(x):
         check(load().collie_gated_forward(
-            ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(wg), ptr(wu), ptr(bg), ptr(bu), n_out,
-            act, ptr(g), ptr(u), ptr(y), stream_ptr()), 'collie_gated_forward')
+            ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), ptr(bg), ptr(bu), n_out, act, ptr(g),
+            ptr(u), ptr(y), ptr(ws), ws.numel(), stream_ptr()), 'collie_gated_forward')
     return y, g, u
 
 
@@ -1175,10 +1180,12 @@ def gated_backward(dy, x, gate_weight, up_weight, activation, kept_gate, kept_up
     if m == 0:
         return tuple(out)
     dy, dy_ld = rows_view(dy, n_out)
-    workspace, need = _layer_workspace(x, m, n_in, n_out, 1)
+    tag = element_type(x, 'x')
+    ws = _workspace(load().collie_layer_backward_workspace_bytes(
+        ptr(dy), dy_ld, ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out, act), x)
     with _on_device(x):
         check(load().collie_gated_backward(
-            ptr(dy), dy_ld, ptr(rows), ld, element_type(x, 'x'), m, n_in, ptr(wg), ptr(wu), n_out,
-            act, ptr(kept_gate), ptr(kept_up), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]),
-            ptr(out[4]), ptr(workspace), need, stream_ptr()), 'collie_gated_backward')
+            ptr(dy), dy_ld, ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out, act,
+            ptr(kept_gate), ptr(kept_up), *[ptr(t) for t in out], ptr(ws), ws.numel(),
+            stream_ptr()), 'collie_gated_backward')
     return tuple(out)

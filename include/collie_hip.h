@@ -852,26 +852,34 @@ enum {
   COLLIE_ACT_GELU = 5        /* z Phi(z), with erf */
 };
 
+/* Workspaces of the two layers (up_weight NULL: the linear one).  They depend on the addresses and
+ * distances of the operands: rows that are no whole aligned 16-byte packs are copied into some. */
+size_t collie_layer_forward_workspace_bytes(const void* x, int64_t x_ld, int32_t dtype, int64_t m,
+                                            int32_t n_in, const void* weight, const void* up_weight,
+                                            int32_t n_out);
+size_t collie_layer_backward_workspace_bytes(const void* dy, int64_t dy_ld, const void* x,
+                                             int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
+                                             const void* weight, const void* up_weight,
+                                             int32_t n_out, int32_t act);
+
 /* y = act(x weight^T + bias) + residual ([m, n_out]); weight [n_out, n_in]; bias / residual may be
  * NULL.  keep [m, n_out] (NULL: not wanted) takes the pre-activations, in x's type (float16:
  * finite ones beyond +-65504 as that), for the backward pass. */
 int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
                           const void* weight, const void* bias, int32_t n_out, int32_t act,
                           const void* residual, int64_t res_ld, void* keep, void* y,
-                          collie_stream_t stream);
+                          void* workspace, size_t workspace_bytes, collie_stream_t stream);
 
 /* y = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias); both biases or none; keep_gate /
  * keep_up as above. */
 int collie_gated_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
                          const void* gate_weight, const void* up_weight, const void* gate_bias,
                          const void* up_bias, int32_t n_out, int32_t act, void* keep_gate,
-                         void* keep_up, void* y, collie_stream_t stream);
+                         void* keep_up, void* y, void* workspace, size_t workspace_bytes,
+                         collie_stream_t stream);
 
 /* Gradients from dy [m, n_out] (that of the residual is dy itself), m >= 1; every output may be NULL
- * (not wanted).  kept_z is NULL for the identity.  workspace:
- * collie_layer_backward_workspace_bytes(dtype, m, n_in, n_out, pair = 0 linear / 1 gated). */
-size_t collie_layer_backward_workspace_bytes(int32_t dtype, int64_t m, int32_t n_in, int32_t n_out,
-                                             int32_t pair);
+ * (not wanted).  kept_z is NULL for the identity. */
 int collie_linear_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int32_t dtype,
                            int64_t m, int32_t n_in, const void* weight, int32_t n_out, int32_t act,
                            const void* kept_z, void* dx, void* dweight, void* dbias, void* workspace,

@@ -292,6 +292,17 @@ def test_gated_activations(kind, dtype):
     run_gated(37, 48, 56, dtype, kind, True, seed=30)
 
 
+# enough 256 x 256 tiles for the large-tile kernel in the forward pass, in dx and in dW
+LARGE = [(4200, 72, 4104), (4200, 4104, 72), (72, 4104, 4200), (4111, 77, 4099)]
+
+
+@pytest.mark.parametrize('dtype', TYPES[1:])
+@pytest.mark.parametrize('m,n_in,n_out', LARGE)
+def test_large_tiles(m, n_in, n_out, dtype):
+    run_linear(m, n_in, n_out, dtype, 'gelu', True, True, seed=40)
+    run_gated(m, n_in, n_out // 2 + 1, dtype, 'silu', True, seed=50)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_layers_take_strides_more_dimensions_and_no_rows(dtype):
     from collie_amd import functional as F

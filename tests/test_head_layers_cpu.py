@@ -82,7 +82,7 @@ def test_rows_view_copies_only_what_it_must():
 def test_c_entry_points_reject_bad_arguments():
     lib = _lib.load()
     p = ctypes.c_void_p(256)            # never dereferenced: every call below is refused
-    none = ctypes.c_void_p(None)
+    none, big = ctypes.c_void_p(None), 1 << 40
     bad = [
         lambda: lib.collie_embedding_rows(p, 9, 4, 4, p, 1, 1, 1.0, p, none, none),
         lambda: lib.collie_embedding_rows(p, 0, 0, 4, p, 1, 1, 1.0, p, none, none),
@@ -104,12 +104,14 @@ def test_c_entry_points_reject_bad_arguments():
         lambda: lib.collie_layer_norm_backward(p, 4, p, 4, 0, 2, 4, p, 0, none, p, p, p, p, p,
                                                1 << 30, none),
         lambda: lib.collie_layer_norm_backward(p, 4, p, 4, 0, 2, 4, p, 0, p, p, p, p, p, p, 4, none),
-        lambda: lib.collie_linear_forward(p, 3, 0, 2, 4, p, p, 5, 0, none, 0, none, p, none),
-        lambda: lib.collie_linear_forward(p, 4, 0, 2, 4, p, p, 5, 6, none, 0, none, p, none),
-        lambda: lib.collie_linear_forward(p, 4, 0, 2, 4, p, p, 5, 0, p, 4, none, p, none),
-        lambda: lib.collie_linear_forward(p, 4, 5, 2, 4, p, p, 5, 0, none, 0, none, p, none),
-        lambda: lib.collie_gated_forward(p, 4, 0, 2, 4, p, p, p, none, 5, 4, none, none, p, none),
-        lambda: lib.collie_gated_forward(p, 4, 0, 2, 4, p, p, none, none, 5, 4, p, none, p, none),
+        lambda: lib.collie_linear_forward(p, 3, 0, 2, 4, p, p, 5, 0, none, 0, none, p, p, big, none),
+        lambda: lib.collie_linear_forward(p, 4, 0, 2, 4, p, p, 5, 6, none, 0, none, p, p, big, none),
+        lambda: lib.collie_linear_forward(p, 4, 0, 2, 4, p, p, 5, 0, p, 4, none, p, p, big, none),
+        lambda: lib.collie_linear_forward(p, 4, 5, 2, 4, p, p, 5, 0, none, 0, none, p, p, big, none),
+        lambda: lib.collie_linear_forward(p, 4, 0, 2, 4, p, p, 5, 0, none, 0, none, p, p, 1, none),
+        lambda: lib.collie_gated_forward(p, 4, 0, 2, 4, p, p, p, p, 5, 4, p, p, p, none, big, none),
+        lambda: lib.collie_gated_forward(p, 4, 0, 2, 4, p, p, p, none, 5, 4, none, none, p, p, big, none),
+        lambda: lib.collie_gated_forward(p, 4, 0, 2, 4, p, p, none, none, 5, 4, p, none, p, p, big, none),
         lambda: lib.collie_linear_backward(p, 5, p, 4, 0, 0, 4, p, 5, 0, none, p, p, p, p, 1 << 30,
                                            none),
         lambda: lib.collie_linear_backward(p, 5, p, 4, 0, 2, 4, p, 5, 4, none, p, p, p, p, 1 << 30,
