@@ -19,38 +19,40 @@ struct Gemm {
   const void* b2;        // second matrix of b's shape, or NULL
   int64_t k_split;       // without kEpiGated: k >= k_split reads b2 at k - k_split, and of either
   int64_t k_valid;       // matrix only the first k_valid are there (the rest is padding: zero)
-  int64_t b2_offset;     // b2 - b, in elements
+  int64_t b2_step;       // from row k_split of b (not there) to row 0 of b2, in elements
   int64_t m, n, k;
-  int64_t k_chunk;       // depth of one of the `splits` parts
+  // the first `full` tiles are computed whole; the depth of the others is cut into `splits` parts of
+  // k_chunk, whose sums go to partial [splits, tiles - full, accumulators, tile rows, tile columns]
+  int64_t full;
   int splits;
+  int64_t k_chunk;
+  float* partial;
   // epilogue
   int act;
   const void *bias, *bias2;
   const void* residual;
   int64_t res_ld;
-  void *keep, *keep2;    // pre-activations for the backward pass [m, n], or NULL
+  void *keep, *keep2;    // pre-activations for the backward pass [m, n], or NULL (gated: float32)
   void *c, *c2;          // output [m, n]; with kEpiStore rows >= row_split are c2's, and of either
   int64_t row_split;     // only the first row_valid are wanted
   int64_t row_valid;
-  float* partial;        // splits > 1: [splits, accumulators, m, n] sums of the parts of the depth
 };
 
-// the sums of one part of the depth
-template <int EPI, int W>
-__device__ __forceinline__ void store_part(const Gemm& g, int64_t row, int64_t col, int64_t part,
-                                           const float (&v)[W], const float (&u)[W]) {
-  if (row >= g.m || col >= g.n) return;
+// biases of the columns col .. col + W
+template <typename T, int EPI, int W>
+__device__ __forceinline__ void load_biases(const Gemm& g, int64_t col, float (&b)[W], float (&b2)[W]) {
+#pragma unroll
+  for (int j = 0; j < W; ++j) b[j] = b2[j] = 0.0f;
+  if (EPI == kEpiStore || g.bias == nullptr || col >= g.n) return;
   const int left = g.n - col < W ? static_cast<int>(g.n - col) : W;
-  constexpr int NB = EPI == kEpiGated ? 2 : 1;
-  float* p = g.partial + part * NB * g.m * g.n + row * g.n + col;
-  store_pack<float, W>(p, left, v);
-  if constexpr (NB == 2) store_pack<float, W>(p + g.m * g.n, left, u);
+  load_pack<T, W>(static_cast<const T*>(g.bias) + col, left, b);
+  if constexpr (EPI == kEpiGated) load_pack<T, W>(static_cast<const T*>(g.bias2) + col, left, b2);
 }
 
 // results at (row, col .. col + W): columns of one row that one thread holds
 template <typename T, int EPI, int W>
 __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t col, float (&v)[W],
-                                           float (&u)[W]) {
+                                           float (&u)[W], const float (&b)[W], const float (&b2)[W]) {
   if (row >= g.m || col >= g.n) return;
   const int left = g.n - col < W ? static_cast<int>(g.n - col) : W;
   const int64_t at = row * g.n + col;
@@ -59,25 +61,20 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
     const int64_t r = row < g.row_split ? row : row - g.row_split;
     if (c && r < g.row_valid) store_pack<T, W>(c + r * g.n + col, left, v);
   } else {
-    float add[W];
-    if (g.bias) {
-      load_pack<T, W>(static_cast<const T*>(g.bias) + col, left, add);
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += add[j];
-      if constexpr (EPI == kEpiGated) {
-        load_pack<T, W>(static_cast<const T*>(g.bias2) + col, left, add);
-#pragma unroll
-        for (int j = 0; j < W; ++j) u[j] += add[j];
-      }
+    for (int j = 0; j < W; ++j) {
+      v[j] += b[j];
+      if (EPI == kEpiGated) u[j] += b2[j];
     }
+    float t[W];
     if (g.keep) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) add[j] = kept<T>(v[j]);
-      store_pack<T, W>(static_cast<T*>(g.keep) + at, left, add);
       if constexpr (EPI == kEpiGated) {
+        store_pack<float, W>(static_cast<float*>(g.keep) + at, left, v);
+        store_pack<float, W>(static_cast<float*>(g.keep2) + at, left, u);
+      } else {
 #pragma unroll
-        for (int j = 0; j < W; ++j) add[j] = kept<T>(u[j]);
-        store_pack<T, W>(static_cast<T*>(g.keep2) + at, left, add);
+        for (int j = 0; j < W; ++j) t[j] = kept<T>(v[j]);
+        store_pack<T, W>(static_cast<T*>(g.keep) + at, left, t);
       }
     }
     act_values(g.act, v);
@@ -85,9 +82,9 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] *= u[j];
     } else if (g.residual) {
-      load_pack<T, W>(static_cast<const T*>(g.residual) + row * g.res_ld + col, left, add);
+      load_pack<T, W>(static_cast<const T*>(g.residual) + row * g.res_ld + col, left, t);
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += add[j];
+      for (int j = 0; j < W; ++j) v[j] += t[j];
     }
     store_pack<T, W>(static_cast<T*>(g.c) + at, left, v);
   }

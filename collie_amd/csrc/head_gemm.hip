@@ -17,7 +17,8 @@ constexpr int kBlock = 256;
 
 // ---- dz = dy f'(z) (linear), [dg | du] (gated), and the column sums for the bias gradients --------
 struct ActBwd {
-  const void *dy, *z, *u;  // z: kept pre-activation (NULL: identity); u: the gated layer's second one
+  const void *dy;
+  const void *z, *u;       // kept pre-activations: of the rows' type (NULL: identity), gated: float32
   void* dz;                // [m, dz_ld]; NULL: only the column sums are wanted
   float* partial;          // [gridDim.y, pair * n] or NULL
   int64_t m, n, dy_ld, dz_ld;
@@ -43,8 +44,9 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
       float dy[V], z[V], d[V], u[V];
       load_pack<T, V>(static_cast<const T*>(p.dy) + row * p.dy_ld + col, left, dy);
       if (p.z) {
-        load_pack<T, V>(static_cast<const T*>(p.z) + row * p.n + col, left, z);
-        if (PAIR) load_pack<T, V>(static_cast<const T*>(p.u) + row * p.n + col, left, u);
+        using K = std::conditional_t<PAIR, float, T>;
+        load_pack<K, V>(static_cast<const K*>(p.z) + row * p.n + col, left, z);
+        if (PAIR) load_pack<K, V>(static_cast<const K*>(p.u) + row * p.n + col, left, u);
         act_slopes(p.act, z, d);
       }
 #pragma unroll
@@ -170,67 +172,83 @@ int lay_out(const void*& p, int64_t& ld, int64_t rows, int64_t cols, void* room,
 constexpr int64_t kSkinnyRows = 64;  // rows of the kernel that streams the weights
 constexpr int64_t kCus = 256;
 
+// A CU holds one workgroup of the 256 x 256 kernel or two of the 128 x 128 one (LDS).  The tiles that
+// fill whole rounds of the chip are computed as they are; those left over are cut along the depth, so
+// that they fill a round too: 344 tiles of 256 (a weight gradient of 11,008 x 2,048 over 16,384 rows)
+// took two rounds, 947 us.  The tile and the number of parts are the ones with the least time by
+// what a workgroup of either kernel was measured to do (products per second on large matrices), what
+// the parts' sums cost in memory traffic and what one more launch does.
 struct Plan {
-  int tile;    // BM = BN
-  int splits;
-  int64_t k_chunk;
+  int tile;  // BM = BN
+  int64_t tiles, full, splits, k_chunk;
 };
 
 template <typename T>
 Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair) {
   const int64_t depth = 128 / static_cast<int64_t>(sizeof(T));
-  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n * (pair ? 2 : 1) + t - 1) / t); };
-  Plan p;
-  // the large tile reads half as much from LDS per product, but one workgroup fills a CU
-  p.tile = sizeof(T) == 2 && tiles(256) >= kCus ? 256 : 128;
-  // too few tiles for the chip: the depth is cut until there are about two workgroups per CU, in
-  // parts of at least four stages
-  int64_t s = (2 * kCus) / tiles(p.tile);
-  if (s > k / (4 * depth)) s = k / (4 * depth);
-  if (s < 1) s = 1;
-  p.k_chunk = ((k + s - 1) / s + depth - 1) / depth * depth;
-  p.splits = static_cast<int>((k + p.k_chunk - 1) / p.k_chunk);
-  if (p.splits < 1) p.splits = 1;
-  return p;
+  const int64_t stages = (k + depth - 1) / depth;
+  const double rate[2] = {sizeof(T) == 2 ? 0.9e15 : 1.6e14, sizeof(T) == 2 ? 1.04e15 : 1.9e14};
+  Plan best;
+  double best_time = 0.0;
+  for (int big = 0; big < 2; ++big) {
+    const int64_t t = big ? 256 : 128, slots = big ? kCus : 2 * kCus;
+    const int64_t tiles = ((m + t - 1) / t) * ((n * (pair ? 2 : 1) + t - 1) / t);
+    const int64_t full = tiles / slots * slots, rest = tiles - full;
+    // of one tile: its products, and two stages' worth for the first load and the epilogue
+    const double one = 2.0 * t * t * static_cast<double>((stages + 2) * depth) * slots / rate[big];
+    for (int64_t q = 0; q <= 4; ++q) {
+      int64_t s = q == 0 || rest == 0 ? 1 : q * slots / rest;
+      if (s > stages / 4) s = stages / 4;
+      if (s < 1) s = 1;
+      const int64_t part = (stages + s - 1) / s;
+      s = (stages + part - 1) / part;
+      double time = one * (full / slots);
+      time += one * ((rest * s + slots - 1) / slots) * (part + 2) / (stages + 2);
+      if (s > 1) time += 5e-6 + 8.0 * s * rest * t * t / 4e12;
+      if ((big == 0 && q == 0) || time < best_time) {
+        best_time = time;
+        best = {static_cast<int>(t), tiles, s > 1 ? full : tiles, s, part * depth};
+      }
+    }
+  }
+  return best;
 }
 
-template <typename T>
-size_t partial_floats(int64_t m, int64_t n, int64_t k, bool pair) {
-  const Plan p = plan_gemm<T>(m, n, k, pair);
-  return p.splits > 1 ? static_cast<size_t>(p.splits) * (pair ? 2 : 1) * m * n : 0;
+size_t partial_floats(const Plan& p) {
+  return static_cast<size_t>(p.splits > 1 ? p.splits * (p.tiles - p.full) * p.tile * p.tile : 0);
+}
+
+template <typename T, int TILE, bool AKC, bool BKC, int EPI, bool CAT>
+int launch_tile(const Gemm& g, const Plan& p, hipStream_t stream) {
+  const int64_t rest = p.tiles - p.full;
+  const int64_t total = p.full + rest * p.splits;
+  COLLIE_REQUIRE(total < (int64_t{1} << 31), "matrix product: too many tiles");
+  constexpr int WN = TILE == 256 ? 4 : 2;
+  hipLaunchKernelGGL((gemm_tile_kernel<T, TILE, TILE, 2, WN, AKC, BKC, EPI, CAT>),
+                     dim3(static_cast<unsigned>(total)), dim3(kWave * 2 * WN), 0, stream, g);
+  if (check_launch("gemm_tile_kernel")) return -2;
+  if (rest == 0) return 0;
+  constexpr int64_t per_tile = TILE * TILE / (EPI == kEpiGated ? 2 : 1) / 4 / kWave;
+  const dim3 grid(static_cast<unsigned>(rest * per_tile));
+  if (p.splits <= 8)
+    hipLaunchKernelGGL((gemm_finish_kernel<T, TILE, EPI, 1>), grid, dim3(kWave), 0, stream, g);
+  else
+    hipLaunchKernelGGL((gemm_finish_kernel<T, TILE, EPI, 8>), grid, dim3(kWave * 8), 0, stream, g);
+  return check_launch("gemm_finish_kernel");
 }
 
 template <typename T, bool AKC, bool BKC, int EPI, bool CAT>
 int launch_tiles(Gemm& g, hipStream_t stream) {
-  constexpr bool PAIR = EPI == kEpiGated;
-  const Plan p = plan_gemm<T>(g.m, g.n, g.k, PAIR);
-  g.splits = p.splits;
+  const Plan p = plan_gemm<T>(g.m, g.n, g.k, EPI == kEpiGated);
+  g.full = p.full;
+  g.splits = static_cast<int>(p.splits);
   g.k_chunk = p.k_chunk;
-  g.b2_offset = g.b2 ? (reinterpret_cast<intptr_t>(g.b2) - reinterpret_cast<intptr_t>(g.b.p)) /
-                           static_cast<intptr_t>(sizeof(T))
-                     : 0;
-  const int64_t tn = PAIR ? p.tile / 2 : p.tile;
-  const int64_t total = ((g.m + p.tile - 1) / p.tile) * ((g.n + tn - 1) / tn) * p.splits;
-  COLLIE_REQUIRE(total < (int64_t{1} << 31), "matrix product: too many tiles");
-  const dim3 grid(static_cast<unsigned>(total));
-  if (p.tile == 256) {
-    if constexpr (sizeof(T) == 2)
-      hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 4, AKC, BKC, EPI, CAT>), grid, dim3(512),
-                         0, stream, g);
-  } else {
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 128, 128, 2, 2, AKC, BKC, EPI, CAT>), grid, dim3(256), 0,
-                       stream, g);
-  }
-  if (check_launch("gemm_tile_kernel")) return -2;
-  if (p.splits == 1) return 0;
-  const int64_t blocks = (g.m * ((g.n + 3) / 4) + kWave - 1) / kWave;
-  if (p.splits <= 8)
-    hipLaunchKernelGGL((gemm_finish_kernel<T, EPI, 1>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(kWave), 0, stream, g);
-  else
-    hipLaunchKernelGGL((gemm_finish_kernel<T, EPI, 8>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(kWave * 8), 0, stream, g);
-  return check_launch("gemm_finish_kernel");
+  if (CAT)
+    g.b2_step = (reinterpret_cast<intptr_t>(g.b2) - reinterpret_cast<intptr_t>(g.b.p)) /
+                    static_cast<intptr_t>(sizeof(T)) -
+                g.k_split * g.b.ks;
+  return p.tile == 256 ? launch_tile<T, 256, AKC, BKC, EPI, CAT>(g, p, stream)
+                       : launch_tile<T, 128, AKC, BKC, EPI, CAT>(g, p, stream);
 }
 
 template <typename T, int EPI>
@@ -276,7 +294,7 @@ FwdWs carve_fwd(void* base, const void* x, int64_t x_ld, int64_t m, int64_t n_in
     if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
     if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
     if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
-    ws.partial = c.take<float>(partial_floats<T>(m, n_out, n_in, w2 != nullptr));
+    ws.partial = c.take<float>(partial_floats(plan_gemm<T>(m, n_out, n_in, w2 != nullptr)));
   }
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;
@@ -304,8 +322,8 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
   if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
   if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
   ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m)) * pair * n_out);
-  const size_t a = partial_floats<T>(m, n_in, (pair - 1) * half + n_out, false);
-  const size_t b = partial_floats<T>((pair - 1) * half + n_out, n_in, m, false);
+  const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false));
+  const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false));
   ws.partial = c.take<float>(a > b ? a : b);
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;
@@ -331,7 +349,6 @@ int layer_forward(const void* x, int64_t x_ld, const void* w, const void* w2, co
   g.m = m;
   g.n = n_out;
   g.k = n_in;
-  g.splits = 1;
   g.act = act;
   g.bias = bias;
   g.bias2 = bias2;

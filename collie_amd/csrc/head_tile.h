@@ -39,25 +39,63 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// A fragment: 16 rows by 32 k (16-bit) or 16 k (float32); lane l holds row l % 16 and
-// k = 8 (l / 16) + j, or 4 (l / 16) + j.
+constexpr int kMfma = 0x008, kDsRead = 0x100;  // groups of __builtin_amdgcn_sched_group_barrier
+
+// A fragment: 16 rows by 32 k; lane l holds row l % 16 and k = 8 (l / 16) + j.
 template <typename T>
 struct Frag {
   s16x8 v;
 };
 template <>
 struct Frag<float> {
-  f32x4 v;
+  float v[8];
 };
+
+// A float32 fragment as three bfloat16 ones, x = hi + mid + lo exactly: 8 significant bits each, what
+// is left after rounding to the nearest.  Of the nine products of two such numbers the six of
+// weight 2^-16 and more are summed; the others are below 2^-23 of the product, which is what float32
+// rounds it by.  Six bfloat16 instructions do 32 k in 96 cycles; the float32 ones need 256.  Values
+// without a finite bfloat16 (infinities, NaN, the top of the range) make sums that are not finite:
+// the tile is then computed again with the float32 instructions (gemm_tile_kernel).  Parts below the
+// smallest normal number are lost, at most 2^-126 times the other factor.
+struct Split {
+  bf16x8 hi, mid, lo;
+};
+template <typename T>
+__device__ __forceinline__ Split split(const Frag<T>& f) {
+  Split s;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s.hi[j] = static_cast<bf16_t>(f.v[j]);
+      const float r = f.v[j] - static_cast<float>(s.hi[j]);
+      s.mid[j] = static_cast<bf16_t>(r);
+      s.lo[j] = static_cast<bf16_t>(r - static_cast<float>(s.mid[j]));
+    }
+  }
+  return s;
+}
+
+__device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void multiply(const Split& a, const Split& b, f32x4& c) {
+  c = mfma_bf16(a.lo, b.hi, c);   // the smallest first
+  c = mfma_bf16(a.hi, b.lo, c);
+  c = mfma_bf16(a.mid, b.mid, c);
+  c = mfma_bf16(a.mid, b.hi, c);
+  c = mfma_bf16(a.hi, b.mid, c);
+  c = mfma_bf16(a.hi, b.hi, c);
+}
 
 template <typename T>
 __device__ __forceinline__ void multiply(const Frag<T>& a, const Frag<T>& b, f32x4& c) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[t], b.v[t], c, 0, 0, 0);
+    for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[t], b.v[t], c, 0, 0, 0);
   } else if constexpr (std::is_same<T, bf16_t>::value) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v),
-                                                __builtin_bit_cast(bf16x8, b.v), c, 0, 0, 0);
+    c = mfma_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c);
   } else {
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v),
                                                __builtin_bit_cast(f16x8, b.v), c, 0, 0, 0);
@@ -74,21 +112,30 @@ struct Image {
   static __device__ __forceinline__ int swizzle(int row) {
     if (KC) return (row >> 1) & 7;
     if (sizeof(T) == 2) return ((row & 3) | ((row >> 1) & 4)) << 1;
-    return ((row >> 2) & 3) << 2;
+    return ((row >> 3) & 3) << 2;
   }
   // image row and source chunk of the 16 bytes at linear position `at`
   static __device__ __forceinline__ void source(int at, int& row, int& chunk) {
     row = at / kRowChunks;
     chunk = (at % kRowChunks) ^ swizzle(row);
   }
-  // fragment `step` (of 2) of the 16 rows from row0 on
+  static constexpr int kSteps = kDepth / 32;  // fragments along the depth
+  // fragment `step` of the 16 rows from row0 on
   static __device__ __forceinline__ Frag<T> read(const char* img, int row0, int step, int lane) {
     const int r = lane & 15, g = lane >> 4;
     Frag<T> f;
-    if constexpr (KC) {
+    if constexpr (KC && sizeof(T) == 2) {
       const int row = row0 + r;
-      const char* p = img + row * 128 + ((4 * step + g) ^ swizzle(row)) * 16;
-      f.v = *reinterpret_cast<const decltype(f.v)*>(p);
+      f.v = *reinterpret_cast<const s16x8*>(img + row * 128 + ((4 * step + g) ^ swizzle(row)) * 16);
+    } else if constexpr (KC) {
+      const int row = row0 + r;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 v =
+            *reinterpret_cast<const f32x4*>(img + row * 128 + ((2 * g + h) ^ swizzle(row)) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.v[4 * h + j] = v[j];
+      }
     } else if constexpr (sizeof(T) == 2) {
       s16x4 part[2];
 #pragma unroll
@@ -102,10 +149,10 @@ struct Image {
       f.v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int k = 16 * step + 4 * g + t;
+      for (int j = 0; j < 8; ++j) {
+        const int k = 8 * g + j;
         const int chunk = (row0 >> 2) + (r >> 2);
-        f.v[t] = *reinterpret_cast<const float*>(img + k * (R * 4) + (chunk ^ swizzle(k)) * 16 +
+        f.v[j] = *reinterpret_cast<const float*>(img + k * (R * 4) + (chunk ^ swizzle(k)) * 16 +
                                                  (r & 3) * 4);
       }
     }
@@ -145,7 +192,7 @@ struct Feed {
         int64_t col = row0 + c * V;
         col = col < end ? col : end - V;
         kk[j] = r;
-        p[j] = static_cast<const T*>(base) + col + (CAT ? 0 : (k0 + r) * ld);
+        p[j] = static_cast<const T*>(base) + col + (k0 + r) * ld;
       }
     }
   }
@@ -158,30 +205,69 @@ struct Feed {
     for (int j = 0; j < N; ++j) {
       const void* q = p[j];
       if constexpr (CAT) {
-        int64_t at = k + kk[j];
+        const int64_t at = k + kk[j];
         const bool second = at >= g.k_split;
-        const bool in = at < k1;
-        if (second) at -= g.k_split;
-        q = p[j] + (second ? g.b2_offset : 0) + at * ld;
-        if (!in || at >= g.k_valid) q = &g_zero_chunk;
+        if (second) q = p[j] + g.b2_step;
+        if (!whole || g.k_valid != g.k_split) {
+          if (at >= k1 || at - (second ? g.k_split : 0) >= g.k_valid) q = &g_zero_chunk;
+        }
       } else {
         if (!whole && k + kk[j] >= k1) q = &g_zero_chunk;
-        p[j] += KC ? static_cast<int64_t>(Img::kDepth) : Img::kDepth * ld;
       }
+      p[j] += KC ? static_cast<int64_t>(Img::kDepth) : Img::kDepth * ld;
       dma16(q, to + j * THREADS * 16);
     }
   }
 };
 
-// Tiles in an order that keeps the operands in the caches: workgroups go round the 8 XCDs, so XCD x
-// gets the x-th run of tiles; inside a run, kBand row tiles by all column tiles.
-__device__ __forceinline__ void tile_of(int64_t id, int64_t total, int64_t tiles_m, int64_t tiles_n,
-                                        int64_t& tm, int64_t& tn, int64_t& part) {
-  constexpr int64_t kBand = 8;
+// Lanes l, l + 16, l + 32, l + 48 hold columns 4 q .. 4 q + 3 (q = l / 16) of one row of two or four
+// 16-column tiles.  Afterwards lane row q holds, of four tiles, all of tile q; of two tiles, the half
+// q / 2 of tile q % 2.
+__device__ __forceinline__ void swap_lanes16(float& a, float& b) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a),
+                                                  __builtin_bit_cast(uint32_t, b), false, false);
+  const uint32_t a1 = s[0], b1 = s[1];  // (a bit_cast of a vector's element would take element 0)
+  a = __builtin_bit_cast(float, a1);
+  b = __builtin_bit_cast(float, b1);
+}
+__device__ __forceinline__ void swap_lanes32(float& a, float& b) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a),
+                                                  __builtin_bit_cast(uint32_t, b), false, false);
+  const uint32_t a1 = s[0], b1 = s[1];  // (a bit_cast of a vector's element would take element 0)
+  a = __builtin_bit_cast(float, a1);
+  b = __builtin_bit_cast(float, b1);
+}
+__device__ __forceinline__ void spread2(const f32x4& t0, const f32x4& t1, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = t0[j];
+    v[4 + j] = t1[j];
+    swap_lanes16(v[j], v[4 + j]);
+  }
+}
+__device__ __forceinline__ void spread4(const f32x4 (&t)[4], float (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[4 * k + j] = t[k][j];
+    swap_lanes32(v[j], v[8 + j]);
+    swap_lanes32(v[4 + j], v[12 + j]);
+    swap_lanes16(v[j], v[4 + j]);
+    swap_lanes16(v[8 + j], v[12 + j]);
+  }
+}
+
+// Workgroups go round the 8 XCDs: XCD x gets the x-th run of the numbers below `total`.
+__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t total) {
   const int64_t q = total / 8, r = total % 8, x = id % 8;
-  id = x * q + (x < r ? x : r) + id / 8;
-  part = id / (tiles_m * tiles_n);
-  id -= part * tiles_m * tiles_n;
+  return x * q + (x < r ? x : r) + id / 8;
+}
+
+// Tile number -> row and column tile: kBand row tiles by all column tiles, then the next band, so
+// that the tiles of a run share operands in their XCD's cache.
+__device__ __forceinline__ void tile_at(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t& tm,
+                                        int64_t& tn) {
+  constexpr int64_t kBand = 8;
   const int64_t band = id / (kBand * tiles_n);
   const int64_t high = tiles_m - band * kBand < kBand ? tiles_m - band * kBand : kBand;
   id -= band * kBand * tiles_n;
@@ -208,73 +294,139 @@ __global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm 
   const int wm = wave / WN, wn = wave % WN;
 
   const int64_t tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + TN - 1) / TN;
-  int64_t tm, tn, part;
-  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn, part);
+  const bool cut = blockIdx.x >= g.full;  // one part of the depth of a tile
+  int64_t id, part = 0, tm, tn;
+  if (cut) {
+    const int64_t rest = tiles_m * tiles_n - g.full;
+    id = xcd_order(blockIdx.x - g.full, rest * g.splits);
+    part = id / rest;
+    id = g.full + id % rest;
+  } else {
+    id = xcd_order(blockIdx.x, g.full);
+  }
+  tile_at(id, tiles_m, tiles_n, tm, tn);
   const int64_t row0 = tm * BM, col0 = tn * TN;
-  const int64_t k0 = part * g.k_chunk;
-  const int64_t k1 = k0 + g.k_chunk < g.k ? k0 + g.k_chunk : g.k;
-
-  Feed<T, BM, AKC, THREADS, false, false> fa;
-  Feed<T, BN, BKC, THREADS, PAIR, CAT> fb;
-  fa.init(g.a.p, nullptr, AKC ? g.a.rs : g.a.ks, row0, g.m, k0, tid);
-  fb.init(g.b.p, g.b2, BKC ? g.b.rs : g.b.ks, col0, g.n, k0, tid);
+  const int64_t k0 = cut ? part * g.k_chunk : 0;
+  const int64_t k1 = cut && k0 + g.k_chunk < g.k ? k0 + g.k_chunk : g.k;
 
   f32x4 acc[MT][NT];
+  // float32: EXACT takes the float32 instructions
+  auto product = [&](auto exact) {
+    constexpr bool EXACT = decltype(exact)::value;
+    Feed<T, BM, AKC, THREADS, false, false> fa;
+    Feed<T, BN, BKC, THREADS, PAIR, CAT> fb;
+    fa.init(g.a.p, nullptr, AKC ? g.a.rs : g.a.ks, row0, g.m, k0, tid);
+    fb.init(g.b.p, g.b2, BKC ? g.b.rs : g.b.ks, col0, g.n, k0, tid);
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  fa.issue(lds0, k0, k1, g);
-  fb.issue(lds0 + ImgA::kBytes, k0, k1, g);
-  int cur = 0;
-  for (int64_t k = k0; k < k1; k += kDepth) {
-    wait_dma();      // this wave's loads of the stage have landed
-    tile_barrier();  // everyone's have, and the other stage has been read
-    if (k + kDepth < k1) {
-      const uint32_t to = lds0 + (cur ^ 1) * kStage;
-      fa.issue(to, k + kDepth, k1, g);
-      fb.issue(to + ImgA::kBytes, k + kDepth, k1, g);
-    }
-    const char* ia = lds + cur * kStage;
-    const char* ib = ia + ImgA::kBytes;
-#pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      Frag<T> b[NT], a[MT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int row = PAIR ? (j / HALF) * (BN / 2) + wn * (TN / WN) + (j % HALF) * 16
-                             : wn * (BN / WN) + j * 16;
-        b[j] = ImgB::read(ib, row, step, lane);
+      for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    fa.issue(lds0, k0, k1, g);
+    fb.issue(lds0 + ImgA::kBytes, k0, k1, g);
+    int cur = 0;
+    for (int64_t k = k0; k < k1; k += kDepth) {
+      wait_dma();      // this wave's loads of the stage have landed
+      tile_barrier();  // everyone's have, and the other stage has been read
+      if (k + kDepth < k1) {
+        const uint32_t to = lds0 + (cur ^ 1) * kStage;
+        fa.issue(to, k + kDepth, k1, g);
+        fb.issue(to + ImgA::kBytes, k + kDepth, k1, g);
       }
+      const char* ia = lds + cur * kStage;
+      const char* ib = ia + ImgA::kBytes;
+      auto b_row = [&](int j) {
+        return PAIR ? (j / HALF) * (BN / 2) + wn * (TN / WN) + (j % HALF) * 16
+                    : wn * (BN / WN) + j * 16;
+      };
+      if constexpr (sizeof(T) == 4 && !EXACT) {
+        Split b[NT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = ImgA::read(ia, wm * (BM / WM) + i * 16, step, lane);
+        for (int j = 0; j < NT; ++j) b[j] = split(ImgB::read(ib, b_row(j), 0, lane));
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i) {
+          const Split a = split(ImgA::read(ia, wm * (BM / WM) + i * 16, 0, lane));
 #pragma unroll
-        for (int j = 0; j < NT; ++j) multiply<T>(b[j], a[i], acc[i][j]);
+          for (int j = 0; j < NT; ++j) multiply(b[j], a, acc[i][j]);
+        }
+      } else {
+#pragma unroll
+        for (int step = 0; step < ImgA::kSteps; ++step) {
+          Frag<T> b[NT], a[MT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) b[j] = ImgB::read(ib, b_row(j), step, lane);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) a[i] = ImgA::read(ia, wm * (BM / WM) + i * 16, step, lane);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) multiply<T>(b[j], a[i], acc[i][j]);
+        }
+        if constexpr (sizeof(T) == 2) {
+          // the order of the above: the fragments of the next row tiles are on their way while those
+          // at hand are multiplied
+          constexpr int RA = AKC ? 1 : 2, RB = BKC ? 1 : 2;  // LDS reads per fragment
+          __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB + 2 * RA, 0);
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+#pragma unroll
+            for (int i = 0; i < MT - 2; ++i) {
+              __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+              __builtin_amdgcn_sched_group_barrier(kDsRead, RA, 0);
+            }
+            if (step == 0) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB / 2 + RA, 0);
+              }
+            } else {
+              __builtin_amdgcn_sched_group_barrier(kMfma, 2 * NT, 0);
+            }
+          }
+        }
+      }
+      cur ^= 1;
     }
-    cur ^= 1;
+  };
+  product(std::false_type{});
+  if constexpr (sizeof(T) == 4) {
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) finite = finite && fabsf(acc[i][j][t]) < INFINITY;
+    if (__syncthreads_or(!finite)) product(std::true_type{});
   }
 
+  // Four neighbouring columns per lane would be stored as pieces of 8 bytes.  The lanes that hold a
+  // row exchange theirs, so that one has W neighbouring columns and a row leaves in whole lines.
+  static_assert(NT == 4, "four column tiles per wave");
+  constexpr int W = PAIR ? 8 : 16;
   const int r = lane & 15, q = lane >> 4;
+  const int lc = PAIR ? wn * (TN / WN) + 16 * (q & 1) + 8 * (q >> 1) : wn * (TN / WN) + 16 * q;
+  float b[W], b2[W];
+  if (!cut) load_biases<T, EPI, W>(g, col0 + lc, b, b2);
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < HALF; ++j) {
-      float v[4], u[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        v[t] = acc[i][j][t];
-        u[t] = PAIR ? acc[i][PAIR ? j + HALF : j][t] : 0.0f;
-      }
-      const int64_t row = row0 + wm * (BM / WM) + i * 16 + r;
-      const int64_t col = col0 + wn * (TN / WN) + j * 16 + 4 * q;
-      if (g.splits > 1)
-        store_part<EPI, 4>(g, row, col, part, v, u);
-      else
-        finish_row<T, EPI, 4>(g, row, col, v, u);
+  for (int i = 0; i < MT; ++i) {
+    const int lr = wm * (BM / WM) + i * 16 + r;
+    float v[W], u[W];
+    if constexpr (PAIR) {
+      spread2(acc[i][0], acc[i][1], v);
+      spread2(acc[i][2], acc[i][3], u);
+    } else {
+      spread4(acc[i], v);
     }
+    if (cut) {
+      const int64_t rest = tiles_m * tiles_n - g.full;
+      float* p = g.partial + ((part * rest + id - g.full) * (PAIR ? 2 : 1) * BM + lr) * TN + lc;
+      store_pack<float, W>(p, W, v);
+      if (PAIR) store_pack<float, W>(p + BM * TN, W, u);
+    } else {
+      finish_row<T, EPI, W>(g, row0 + lr, col0 + lc, v, u, b, b2);
+    }
+  }
 }
 
 // The product of at most 16 MT rows, where reading the weights is all there is to it: a workgroup of
@@ -287,7 +439,7 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
   constexpr bool PAIR = EPI == kEpiGated;
   constexpr int NB = PAIR ? 2 : 1;
   constexpr int V = kVec<T>;
-  constexpr int kStep = 4 * V;   // k per fragment
+  constexpr int kStep = 32;      // k per fragment
   constexpr int kRun = 2;        // fragments a wave takes in a row
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 15, q = lane >> 4;
@@ -308,20 +460,24 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   auto load = [&](const T* p, int64_t k) {
     Frag<T> f;
-    if constexpr (WHOLE) {
-      const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(p + (k < g.k ? k : 0));
-      f.v = __builtin_bit_cast(decltype(f.v), v);
-      if (k >= g.k) f.v = decltype(f.v){};
-    } else {
-      Pack<T, V> v;
-      if (k + V <= g.k) {
-        v = *reinterpret_cast<const Pack<T, V>*>(p + k);
+    T v[8];
+#pragma unroll
+    for (int h = 0; h < 8; h += V) {
+      Pack<T, V> pack;
+      if constexpr (WHOLE) {
+        pack = *reinterpret_cast<const Pack<T, V>*>(p + (k + h < g.k ? k + h : 0));
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[h + j] = k + h < g.k ? pack.v[j] : static_cast<T>(0.0f);
+      } else if (k + h + V <= g.k) {
+        pack = *reinterpret_cast<const Pack<T, V>*>(p + k + h);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[h + j] = pack.v[j];
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v.v[j] = k + j < g.k ? p[k + j] : static_cast<T>(0.0f);
+        for (int j = 0; j < V; ++j) v[h + j] = k + h + j < g.k ? p[k + h + j] : static_cast<T>(0.0f);
       }
-      f.v = __builtin_bit_cast(decltype(f.v), v);
     }
+    __builtin_memcpy(&f.v, v, sizeof(v));
     return f;
   };
 #pragma unroll 2
@@ -329,7 +485,7 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
     Frag<T> b[kRun][NB], a[kRun][MT];
 #pragma unroll
     for (int s = 0; s < kRun; ++s) {
-      const int64_t at = k + s * kStep + q * V;
+      const int64_t at = k + s * kStep + q * 8;
 #pragma unroll
       for (int j = 0; j < NB; ++j) b[s][j] = load(w[j], at);
 #pragma unroll
@@ -348,6 +504,8 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
 #pragma unroll
     for (int j = 0; j < NB; ++j) sums[wave][i][j][lane] = acc[i][j];
   __syncthreads();
+  float bias[4], bias2[4];
+  load_biases<T, EPI, 4>(g, col0 + 4 * q, bias, bias2);
   for (int i = wave; i < MT; i += kSkinnyWaves) {
     float v[4], u[4];
 #pragma unroll
@@ -359,53 +517,57 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
         if (PAIR) u[t] += sums[s][i][PAIR ? 1 : 0][lane][t];
       }
     }
-    finish_row<T, EPI, 4>(g, i * 16 + r, col0 + 4 * q, v, u);
+    finish_row<T, EPI, 4>(g, i * 16 + r, col0 + 4 * q, v, u, bias, bias2);
   }
 }
 
-// The parts of the depth added in order, then the epilogue.  64 x 4 results per workgroup; with
-// SLICES > 1 the parts are shared out over the waves, whose sums are added in order through LDS.
-template <typename T, int EPI, int SLICES>
+// The parts of the depth of the cut tiles added in order, then the epilogue: 64 x 4 results of one
+// tile per workgroup; with SLICES > 1 the parts are shared out over the waves, whose sums are added
+// in order through LDS.
+template <typename T, int TILE, int EPI, int SLICES>
 __global__ __launch_bounds__(kWave* SLICES) void gemm_finish_kernel(const Gemm g) {
   constexpr int NB = EPI == kEpiGated ? 2 : 1;
+  constexpr int TN = TILE / NB;
+  constexpr int kPacks = TILE * TN / 4;
   const int lane = threadIdx.x & (kWave - 1), slice = threadIdx.x / kWave;
-  const int64_t packs = (g.n + 3) / 4;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWave + lane;
-  const int64_t row = at / packs, col = (at - row * packs) * 4;
-  const bool in = row < g.m;
-  const int left = in ? static_cast<int>(g.n - col < 4 ? g.n - col : 4) : 0;
-  float v[2][4];
+  const int64_t tiles_m = (g.m + TILE - 1) / TILE, tiles_n = (g.n + TN - 1) / TN;
+  const int64_t rest = tiles_m * tiles_n - g.full;
+  const int64_t tile = blockIdx.x / (kPacks / kWave);
+  const int pack = blockIdx.x % (kPacks / kWave) * kWave + lane;
+  const int lr = pack / (TN / 4), lc = pack % (TN / 4) * 4;
+  int64_t tm, tn;
+  tile_at(g.full + tile, tiles_m, tiles_n, tm, tn);
+  const int64_t row = tm * TILE + lr, col = tn * TN + lc;
+  const float* p = g.partial + (tile * NB * TILE + lr) * TN + lc;
+  f32x4 sum[NB];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[0][j] = v[1][j] = 0.0f;
-  if (in) {
-    const float* p = g.partial + row * g.n + col;
+  for (int b = 0; b < NB; ++b) sum[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (row < g.m && col < g.n) {
 #pragma unroll 4
-    for (int s = slice; s < g.splits; s += SLICES) {
-      float t[4];
+    for (int s = slice; s < g.splits; s += SLICES)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        load_pack<float, 4>(p + (static_cast<int64_t>(s) * NB + b) * g.m * g.n, left, t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[b][j] += t[j];
-      }
-    }
+      for (int b = 0; b < NB; ++b)
+        sum[b] += *reinterpret_cast<const f32x4*>(p + (s * rest * NB + b) * TILE * TN);
   }
   if constexpr (SLICES > 1) {
-    __shared__ float sh[SLICES][NB][kWave][4];
+    __shared__ f32x4 sh[SLICES][NB][kWave];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sh[slice][b][lane][j] = v[b][j];
+    for (int b = 0; b < NB; ++b) sh[slice][b][lane] = sum[b];
     __syncthreads();
     if (slice != 0) return;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int s = 1; s < SLICES; ++s) v[b][j] += sh[s][b][lane][j];
+      for (int s = 1; s < SLICES; ++s) sum[b] += sh[s][b][lane];
   }
-  if (in) finish_row<T, EPI, 4>(g, row, col, v[0], v[1]);
+  float v[4], u[4], bias[4], bias2[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = sum[0][j];
+    u[j] = sum[NB - 1][j];
+  }
+  load_biases<T, EPI, 4>(g, col, bias, bias2);
+  finish_row<T, EPI, 4>(g, row, col, v, u, bias, bias2);
 }
 
 }  // namespace collie

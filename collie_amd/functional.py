@@ -37,7 +37,11 @@ class _EmbeddingRows(torch.autograd.Function):
                 live = flat != padding_idx
                 flat, vals = flat[live], vals[live]
             return torch.sparse_coo_tensor(flat.reshape(1, -1), vals, shape), *[None] * 5
-        return _EmbeddingRowsGrad.apply(dy, ids, shape[0], scale, padding_idx, status), *[None] * 5
+        if torch.is_grad_enabled():         # create_graph: the gradient is differentiated again
+            dw = _EmbeddingRowsGrad.apply(dy, ids, shape[0], scale, padding_idx, status)
+        else:
+            dw = ops.embedding_rows_grad(ids, dy, shape[0], scale, padding_idx, status)
+        return dw, None, None, None, None, None
 
 
 class _EmbeddingRowsGrad(torch.autograd.Function):
@@ -78,16 +82,15 @@ def embedding_rows(weight, ids, scale=1.0, padding_idx=None, sparse=False, statu
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = ops.layer_norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        return *ops.layer_norm_backward(dy, x, weight, bias, mean, rstd,
-                                        ctx.needs_input_grad[:3]), None
+        x, weight, bias, stats = ctx.saved_tensors
+        return *ops.layer_norm_backward(dy, x, weight, bias, stats, ctx.needs_input_grad[:3]), None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

@@ -2,7 +2,6 @@
 Thin tensor-level wrappers over the C ABI: they only marshal torch tensors (device pointers,
 current HIP stream) into ``libcollie_hip.so`` calls.  No arithmetic happens in this file.
 """
-import contextlib
 import ctypes
 from ctypes import byref, c_void_p
 
@@ -931,14 +930,27 @@ def eval_merge_topk(cand_scores, cand_ids, k):
 
 
 # ---- layers of a deeper ranking head ---------------------------------------------------------------
-_ON_CURRENT = contextlib.nullcontext()
+# These calls are short (a training step of a small batch makes many): pointers go to the entry
+# points as plain integers, and the backward forms rely on the checks of the forward ones.
+_cuda_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _on_device(t):
-    """Context in which ``t``'s device is the current one (whose stream the launches take)."""
-    if t.device.index == torch.cuda.current_device():
-        return _ON_CURRENT
-    return torch.cuda.device(t.device)
+def _call(t, name, *args):
+    """Entry point ``name`` on ``t``'s device and that device's current stream."""
+    index = t.get_device()
+    fn = getattr(load(), name)
+    if index == _cuda_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def element_type(t, what):
@@ -951,12 +963,16 @@ def element_type(t, what):
 def rows_view(t, width):
     """``t`` as [rows, width] with contiguous rows that do not overlap (a copy only if it must be),
     and the distance of its rows in elements."""
-    if not t.is_contiguous():
-        if t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
-            t = t.contiguous()
-    if t.dim() != 2:
-        t = t.reshape(-1, width)
+    if t.is_contiguous():
+        return (t if t.dim() == 2 else t.reshape(-1, width)), width
+    if t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        return t.contiguous().reshape(-1, width), width
     return t, (t.stride(0) if t.shape[0] > 1 else width)
+
+
+def _workspace(need, like):
+    """Scratch of one call (its caller holds it until the launches are in the stream)."""
+    return torch.empty(need, dtype=torch.uint8, device=like.device)
 
 
 def embedding_rows(table, ids, scale=1.0, status=None):
@@ -969,11 +985,10 @@ def embedding_rows(table, ids, scale=1.0, status=None):
     if ids.device != table.device:
         raise _lib.CollieHipError(f'ids are on {ids.device}, the table is on {table.device}')
     table, ids = table.contiguous(), ids.contiguous()
-    out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
-    with _on_device(table):
-        check(load().collie_embedding_rows(
-            ptr(table), tag, table.shape[0], table.shape[1], ptr(ids), idx_dtype(ids), ids.numel(),
-            float(scale), ptr(out), ptr(status), stream_ptr()), 'collie_embedding_rows')
+    rows, dim = table.shape
+    out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=table.device)
+    _call(table, 'collie_embedding_rows', table.data_ptr(), tag, rows, dim, ids.data_ptr(),
+          idx_dtype(ids), ids.numel(), scale, out.data_ptr(), _at(status))
     return out
 
 
@@ -991,38 +1006,25 @@ def embedding_rows_grad(ids, dy, num_rows, scale=1.0, padding_idx=None, status=N
     n = ids.numel()
     ids = ids.contiguous()
     dy, ld = rows_view(dy, dim)
-    grad = torch.empty(num_rows, dim, dtype=dy.dtype, device=dy.device)
-    need = int(load().collie_embedding_rows_grad_workspace_bytes(n, dim))
-    workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    with _on_device(dy):
-        check(load().collie_embedding_rows_grad(
-            ptr(ids), idx_dtype(ids), n, ptr(dy), ld, tag, num_rows, dim, float(scale),
-            -1 if padding_idx is None else int(padding_idx), ptr(grad), ptr(workspace), need,
-            ptr(status), stream_ptr()), 'collie_embedding_rows_grad')
+    grad = torch.empty((num_rows, dim), dtype=dy.dtype, device=dy.device)
+    ws = _workspace(load().collie_embedding_rows_grad_workspace_bytes(n, dim), dy)
+    _call(dy, 'collie_embedding_rows_grad', ids.data_ptr(), idx_dtype(ids), n, dy.data_ptr(), ld, tag,
+          num_rows, dim, scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(),
+          ws.data_ptr(), ws.numel(), _at(status))
     return grad
 
 
 def _param(t, like, shape, what, other=None):
-    """A parameter of a layer: on ``like``'s device, of its type (or ``other``'s), contiguous."""
+    """A parameter of a layer: on ``like``'s device, of its type (or ``other``), contiguous."""
     if t is None:
         return None
-    if tuple(t.shape) != shape:
-        raise ValueError(f'{what} must have shape {shape}, not {tuple(t.shape)}')
+    if t.shape != shape:
+        raise ValueError(f'{what} must have shape {tuple(shape)}, not {tuple(t.shape)}')
     if t.device != like.device:
         raise _lib.CollieHipError(f'{what} is on {t.device}, x is on {like.device}')
     if t.dtype != like.dtype and t.dtype != other:
         raise _lib.CollieHipError(f'{what} is {t.dtype}, x is {like.dtype}')
     return t.contiguous()
-
-
-def _norm_params(x, weight, bias):
-    dim = x.shape[-1]
-    weight = _param(weight, x, (dim,), 'weight', torch.float32)
-    bias = _param(bias, x, (dim,), 'bias', torch.float32)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise _lib.CollieHipError(f'weight is {weight.dtype}, bias is {bias.dtype}')
-    given = weight if weight is not None else bias
-    return weight, bias, element_type(given if given is not None else x, 'weight')
 
 
 def layer_norm_forward(x, weight, bias, eps, keep):
@@ -1033,38 +1035,41 @@ def layer_norm_forward(x, weight, bias, eps, keep):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'x must have a last dimension to normalise, not {tuple(x.shape)}')
     dim = x.shape[-1]
-    weight, bias, w_tag = _norm_params(x, weight, bias)
+    weight = _param(weight, x, (dim,), 'weight', torch.float32)
+    bias = _param(bias, x, (dim,), 'bias', torch.float32)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise _lib.CollieHipError(f'weight is {weight.dtype}, bias is {bias.dtype}')
     rows, ld = rows_view(x, dim)
     m = rows.shape[0]
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if keep:
-        mean = torch.empty(m, dtype=torch.float32, device=x.device)
-        rstd = torch.empty(m, dtype=torch.float32, device=x.device)
-    with _on_device(x):
-        check(load().collie_layer_norm_forward(
-            ptr(rows), ld, tag, m, dim, ptr(weight), ptr(bias), w_tag, float(eps), ptr(y),
-            ptr(mean), ptr(rstd), stream_ptr()), 'collie_layer_norm_forward')
-    return y, mean, rstd
+    stats = torch.empty((2, m), dtype=torch.float32, device=x.device) if keep else None
+    _call(x, 'collie_layer_norm_forward', rows.data_ptr(), ld, tag, m, dim, _at(weight), _at(bias),
+          _norm_param_tag(weight, bias, tag), eps, y.data_ptr(), _at(stats),
+          stats.data_ptr() + 4 * m if keep else None)
+    return y, stats
 
 
-def layer_norm_backward(dy, x, weight, bias, mean, rstd, want):
-    """(dx, dweight, dbias) of ``collie_layer_norm_backward``, each None unless ``want`` says so."""
+def _norm_param_tag(weight, bias, tag):
+    given = weight if weight is not None else bias
+    return tag if given is None else _lib.ELEMENT_TYPES[given.dtype]
+
+
+def layer_norm_backward(dy, x, weight, bias, stats, want):
+    """(dx, dweight, dbias) of ``collie_layer_norm_backward`` from a forward call's arguments and
+    statistics, each None unless ``want`` says so."""
     dim = x.shape[-1]
-    weight, bias, w_tag = _norm_params(x, weight, bias)
     rows, ld = rows_view(x, dim)
-    g, g_ld = rows_view(dy, dim)
+    dy, dy_ld = rows_view(dy, dim)
     m = rows.shape[0]
+    tag = _lib.ELEMENT_TYPES[x.dtype]
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
-    dw = torch.empty_like(weight) if want[1] and weight is not None else None
-    db = torch.empty_like(bias) if want[2] and bias is not None else None
-    need = int(load().collie_layer_norm_backward_workspace_bytes(m, dim))
-    workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    with _on_device(x):
-        check(load().collie_layer_norm_backward(
-            ptr(g), g_ld, ptr(rows), ld, element_type(x, 'x'), m, dim, ptr(weight), w_tag, ptr(mean),
-            ptr(rstd), ptr(dx), ptr(dw), ptr(db), ptr(workspace), need, stream_ptr()),
-            'collie_layer_norm_backward')
+    dw, db = (torch.empty((dim,), dtype=p.dtype, device=x.device) if w and p is not None else None
+              for w, p in zip(want[1:], (weight, bias)))
+    ws = _workspace(load().collie_layer_norm_backward_workspace_bytes(m, dim), x)
+    _call(x, 'collie_layer_norm_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, dim,
+          _at(weight.contiguous() if weight is not None else None),
+          _norm_param_tag(weight, bias, tag), stats.data_ptr(), stats.data_ptr() + 4 * m, _at(dx),
+          _at(dw), _at(db), ws.data_ptr(), ws.numel())
     return dx, dw, db
 
 
@@ -1076,46 +1081,25 @@ def activation_code(name):
 
 
 def _layer_args(x, weight, biases, second=None):
-    """Checked (rows of x, their distance, weights, biases, m, n_in, n_out) of a layer."""
+    """Checked (element type, rows of x, their distance, weights, biases) of a layer."""
     require_hip(x, 'x')
-    element_type(x, 'x')
+    tag = element_type(x, 'x')
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f'x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit: expected '
                          'x [..., n_in] and weight [n_out, n_in]')
     n_out, n_in = weight.shape
     if n_out < 1 or n_in < 1:
         raise ValueError(f'weight {tuple(weight.shape)} is empty')
-    weights = [_param(weight, x, (n_out, n_in), 'weight')]
+    weights = [_param(weight, x, weight.shape, 'weight')]
     if second is not None:
-        weights.append(_param(second, x, (n_out, n_in), 'weight'))
+        weights.append(_param(second, x, weight.shape, 'weight'))
     biases = [_param(b, x, (n_out,), 'bias') for b in biases]
     rows, ld = rows_view(x, n_in)
-    return rows, ld, weights, biases, rows.shape[0], n_in, n_out
-
-
-def linear_forward(x, weight, bias, activation, residual, keep):
-    """(y, kept pre-activations or None) of ``collie_linear_forward``."""
-    act = activation_code(activation)
-    rows, ld, (weight,), (bias,), m, n_in, n_out = _layer_args(x, weight, (bias,))
-    shape = (*x.shape[:-1], n_out)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    res, res_ld = None, 0
-    if residual is not None:
-        res = _param_rows(residual, x, shape, 'residual')
-        res, res_ld = rows_view(res, n_out)
-    kept = torch.empty(m, n_out, dtype=x.dtype, device=x.device) if keep and act else None
-    tag = element_type(x, 'x')
-    ws = _workspace(load().collie_layer_forward_workspace_bytes(
-        ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(None), n_out), x)
-    with _on_device(x):
-        check(load().collie_linear_forward(
-            ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(bias), n_out, act, ptr(res), res_ld,
-            ptr(kept), ptr(y), ptr(ws), ws.numel(), stream_ptr()), 'collie_linear_forward')
-    return y, kept
+    return tag, rows, ld, weights, biases
 
 
 def _param_rows(t, like, shape, what):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'{what} must have shape {tuple(shape)}, not {tuple(t.shape)}')
     if t.device != like.device or t.dtype != like.dtype:
         raise _lib.CollieHipError(f'{what} is {t.dtype} on {t.device}, x is {like.dtype} on '
@@ -1123,27 +1107,45 @@ def _param_rows(t, like, shape, what):
     return t
 
 
-def _workspace(need, like):
-    return torch.empty(int(need), dtype=torch.uint8, device=like.device)
+def linear_forward(x, weight, bias, activation, residual, keep):
+    """(y, kept pre-activations or None) of ``collie_linear_forward``."""
+    act = activation_code(activation)
+    tag, rows, ld, (weight,), (bias,) = _layer_args(x, weight, (bias,))
+    n_out, n_in = weight.shape
+    m = rows.shape[0]
+    shape = (*x.shape[:-1], n_out)
+    res, res_ld = None, 0
+    if residual is not None:
+        res, res_ld = rows_view(_param_rows(residual, x, shape, 'residual'), n_out)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    kept = torch.empty((m, n_out), dtype=x.dtype, device=x.device) if keep and act else None
+    ws = _workspace(load().collie_layer_forward_workspace_bytes(
+        rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), None, n_out), x)
+    _call(x, 'collie_linear_forward', rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), _at(bias),
+          n_out, act, _at(res), res_ld, _at(kept), y.data_ptr(), ws.data_ptr(), ws.numel())
+    return y, kept
 
 
 def linear_backward(dy, x, weight, activation, kept, want):
-    """(dx, dweight, dbias) of ``collie_linear_backward``, each None unless ``want`` says so."""
-    act = activation_code(activation)
-    rows, ld, (weight,), _, m, n_in, n_out = _layer_args(x, weight, ())
+    """(dx, dweight, dbias) of ``collie_linear_backward`` from a forward call's arguments and what it
+    kept, each None unless ``want`` says so."""
+    n_out, n_in = weight.shape
+    rows, ld = rows_view(x, n_in)
+    m = rows.shape[0]
+    make = torch.empty if m else torch.zeros
+    dx, dw, db = (make(s, dtype=x.dtype, device=x.device) if w else None for w, s in
+                  zip(want, (x.shape, (n_out, n_in), (n_out,))))
     if m == 0:
-        return tuple(torch.zeros(s, dtype=x.dtype, device=x.device) if w else None for w, s in
-                     zip(want, (x.shape, weight.shape, (n_out,))))
-    g, g_ld = rows_view(dy, n_out)
-    dx, dw, db = (torch.empty(s, dtype=x.dtype, device=x.device) if w else None for w, s in
-                  zip(want, (x.shape, weight.shape, (n_out,))))
-    tag = element_type(x, 'x')
+        return dx, dw, db
+    weight = weight.contiguous()
+    dy, dy_ld = rows_view(dy, n_out)
+    tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
     ws = _workspace(load().collie_layer_backward_workspace_bytes(
-        ptr(g), g_ld, ptr(rows), ld, tag, m, n_in, ptr(weight), ptr(None), n_out, act), x)
-    with _on_device(x):
-        check(load().collie_linear_backward(
-            ptr(g), g_ld, ptr(rows), ld, tag, m, n_in, ptr(weight), n_out, act, ptr(kept), ptr(dx),
-            ptr(dw), ptr(db), ptr(ws), ws.numel(), stream_ptr()), 'collie_linear_backward')
+        dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), None, n_out,
+        act), x)
+    _call(x, 'collie_linear_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
+          weight.data_ptr(), n_out, act, _at(kept), _at(dx), _at(dw), _at(db),
+          ws.data_ptr(), ws.numel())
     return dx, dw, db
 
 
@@ -1152,40 +1154,38 @@ def gated_forward(x, gate_weight, up_weight, gate_bias, up_bias, activation, kee
     act = activation_code(activation)
     if (gate_bias is None) != (up_bias is None):
         raise ValueError('gate_bias and up_bias: both or none')
-    rows, ld, (wg, wu), (bg, bu), m, n_in, n_out = _layer_args(x, gate_weight,
-                                                               (gate_bias, up_bias), up_weight)
-    y = torch.empty(*x.shape[:-1], n_out, dtype=x.dtype, device=x.device)
+    tag, rows, ld, (wg, wu), (bg, bu) = _layer_args(x, gate_weight, (gate_bias, up_bias), up_weight)
+    n_out, n_in = wg.shape
+    m = rows.shape[0]
+    y = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=x.device)
     g = u = None
     if keep:
-        g = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
-        u = torch.empty(m, n_out, dtype=x.dtype, device=x.device)
-    tag = element_type(x, 'x')
+        g, u = torch.empty((2, m, n_out), dtype=torch.float32, device=x.device)
     ws = _workspace(load().collie_layer_forward_workspace_bytes(
-        ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out), x)
-    with _on_device(x):
-        check(load().collie_gated_forward(
-            ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), ptr(bg), ptr(bu), n_out, act, ptr(g),
-            ptr(u), ptr(y), ptr(ws), ws.numel(), stream_ptr()), 'collie_gated_forward')
+        rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(), n_out), x)
+    _call(x, 'collie_gated_forward', rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(),
+          _at(bg), _at(bu), n_out, act, _at(g), _at(u), y.data_ptr(), ws.data_ptr(), ws.numel())
     return y, g, u
 
 
 def gated_backward(dy, x, gate_weight, up_weight, activation, kept_gate, kept_up, want):
-    """(dx, dgate_weight, dup_weight, dgate_bias, dup_bias) of ``collie_gated_backward``, each None
-    unless ``want`` says so."""
-    act = activation_code(activation)
-    rows, ld, (wg, wu), _, m, n_in, n_out = _layer_args(x, gate_weight, (), up_weight)
-    shapes = (x.shape, wg.shape, wu.shape, (n_out,), (n_out,))
-    make = torch.zeros if m == 0 else torch.empty
+    """(dx, dgate_weight, dup_weight, dgate_bias, dup_bias) of ``collie_gated_backward`` from a
+    forward call's arguments and what it kept, each None unless ``want`` says so."""
+    n_out, n_in = gate_weight.shape
+    rows, ld = rows_view(x, n_in)
+    m = rows.shape[0]
+    make = torch.empty if m else torch.zeros
+    shapes = (x.shape, (n_out, n_in), (n_out, n_in), (n_out,), (n_out,))
     out = [make(s, dtype=x.dtype, device=x.device) if w else None for w, s in zip(want, shapes)]
     if m == 0:
-        return tuple(out)
+        return out
+    wg, wu = gate_weight.contiguous(), up_weight.contiguous()
     dy, dy_ld = rows_view(dy, n_out)
-    tag = element_type(x, 'x')
+    tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
     ws = _workspace(load().collie_layer_backward_workspace_bytes(
-        ptr(dy), dy_ld, ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out, act), x)
-    with _on_device(x):
-        check(load().collie_gated_backward(
-            ptr(dy), dy_ld, ptr(rows), ld, tag, m, n_in, ptr(wg), ptr(wu), n_out, act,
-            ptr(kept_gate), ptr(kept_up), *[ptr(t) for t in out], ptr(ws), ws.numel(),
-            stream_ptr()), 'collie_gated_backward')
-    return tuple(out)
+        dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(), n_out,
+        act), x)
+    _call(x, 'collie_gated_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
+          wg.data_ptr(), wu.data_ptr(), n_out, act, kept_gate.data_ptr(), kept_up.data_ptr(),
+          *[_at(t) for t in out], ws.data_ptr(), ws.numel())
+    return out

@@ -871,7 +871,7 @@ int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m,
                           void* workspace, size_t workspace_bytes, collie_stream_t stream);
 
 /* y = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias); both biases or none; keep_gate /
- * keep_up as above. */
+ * keep_up [m, n_out] (NULL: not wanted) take the two pre-activations in float32. */
 int collie_gated_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
                          const void* gate_weight, const void* up_weight, const void* gate_bias,
                          const void* up_bias, int32_t n_out, int32_t act, void* keep_gate,
