@@ -19,7 +19,6 @@ struct Gemm {
   const void* b2;        // second matrix of b's shape, or NULL
   int64_t k_split;       // without kEpiGated: k >= k_split reads b2 at k - k_split, and of either
   int64_t k_valid;       // matrix only the first k_valid are there (the rest is padding: zero)
-  int64_t b2_step;       // from row k_split of b (not there) to row 0 of b2, in elements
   int64_t m, n, k;
   // the first `full` tiles are computed whole; the depth of the others is cut into `splits` parts of
   // k_chunk, whose sums go to partial [splits, tiles - full, accumulators, tile rows, tile columns]

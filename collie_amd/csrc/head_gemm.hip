@@ -145,7 +145,8 @@ __global__ __launch_bounds__(kBlock) void pack_rows_kernel(const T* __restrict__
 
 template <typename T>
 bool whole_packs(const void* p, int64_t ld, int64_t cols) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % kVec<T> == 0 && cols % kVec<T> == 0;
+  // (a stage's loads have 32-bit offsets from its first row)
+  return ld * static_cast<int64_t>(sizeof(T)) < (int64_t{1} << 23) && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % kVec<T> == 0 && cols % kVec<T> == 0;
 }
 
 // columns of a row of whole packs
@@ -222,10 +223,11 @@ template <typename T, int TILE, bool AKC, bool BKC, int EPI, bool CAT>
 int launch_tile(const Gemm& g, const Plan& p, hipStream_t stream) {
   const int64_t rest = p.tiles - p.full;
   const int64_t total = p.full + rest * p.splits;
-  COLLIE_REQUIRE(total < (int64_t{1} << 31), "matrix product: too many tiles");
   constexpr int WN = TILE == 256 ? 4 : 2;
+  const int64_t slots = TILE == 256 ? kCus : 2 * kCus;
   hipLaunchKernelGGL((gemm_tile_kernel<T, TILE, TILE, 2, WN, AKC, BKC, EPI, CAT>),
-                     dim3(static_cast<unsigned>(total)), dim3(kWave * 2 * WN), 0, stream, g);
+                     dim3(static_cast<unsigned>(total < slots ? total : slots)),
+                     dim3(kWave * 2 * WN), 0, stream, g);
   if (check_launch("gemm_tile_kernel")) return -2;
   if (rest == 0) return 0;
   constexpr int64_t per_tile = TILE * TILE / (EPI == kEpiGated ? 2 : 1) / 4 / kWave;
@@ -243,10 +245,6 @@ int launch_tiles(Gemm& g, hipStream_t stream) {
   g.full = p.full;
   g.splits = static_cast<int>(p.splits);
   g.k_chunk = p.k_chunk;
-  if (CAT)
-    g.b2_step = (reinterpret_cast<intptr_t>(g.b2) - reinterpret_cast<intptr_t>(g.b.p)) /
-                    static_cast<intptr_t>(sizeof(T)) -
-                g.k_split * g.b.ks;
   return p.tile == 256 ? launch_tile<T, 256, AKC, BKC, EPI, CAT>(g, p, stream)
                        : launch_tile<T, 128, AKC, BKC, EPI, CAT>(g, p, stream);
 }
@@ -269,11 +267,15 @@ int launch_skinny(const Gemm& g, hipStream_t stream) {
   return -1;
 }
 
-// rows per slice of the column sums, and slices
-constexpr int64_t kActParts = 512;
-int64_t act_parts(int64_t m) {
-  const int64_t parts = (m + 4 * kActRows - 1) / (4 * kActRows);
-  return parts < kActParts ? parts : kActParts;
+// slices of the rows for the column sums: together with the column blocks about sixteen workgroups per
+// CU (with two, 720,896 x 128 float32 ran at 2.8 of the 4.7 TB/s a copy reaches), each of at least
+// four rows per lane group
+int64_t act_parts(int64_t m, int64_t n, int64_t v) {
+  const int64_t columns = (n + kActLanes * v - 1) / (kActLanes * v);
+  int64_t parts = (4096 + columns - 1) / columns;
+  if (parts < 64) parts = 64;
+  const int64_t most = (m + 4 * kActRows - 1) / (4 * kActRows);
+  return parts < most ? parts : most;
 }
 
 // Workspaces.  An operand's room is there only if the operand is not in whole packs already.
@@ -321,7 +323,7 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
   if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
   if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
   if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
-  ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m)) * pair * n_out);
+  ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m, n_out, kVec<T>)) * pair * n_out);
   const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false));
   const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false));
   ws.partial = c.take<float>(a > b ? a : b);
@@ -331,8 +333,8 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
 
 int check_layer(const char* who, int64_t m, int32_t n_in, int32_t n_out, int64_t x_ld, int32_t act) {
   COLLIE_REQUIRE(m >= 0 && m < (int64_t{1} << 31), "%s: bad number of rows", who);
-  COLLIE_REQUIRE(n_in >= 1 && n_out >= 1 && n_in <= (1 << 20) && n_out <= (1 << 20),
-                 "%s: widths must be in [1, 2^20]", who);
+  COLLIE_REQUIRE(n_in >= 1 && n_out >= 1 && n_in <= (1 << 19) && n_out <= (1 << 19),
+                 "%s: widths must be in [1, 2^19]", who);
   COLLIE_REQUIRE(m <= 1 || x_ld >= n_in, "%s: rows of x overlap", who);
   COLLIE_REQUIRE(act >= COLLIE_ACT_IDENTITY && act <= COLLIE_ACT_GELU, "%s: unknown activation %d",
                  who, act);
@@ -401,7 +403,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
       dz_ld = p.dz_ld = wide * half;
     }
     p.partial = sums ? ws.act_partial : nullptr;
-    const int64_t parts = act_parts(m);
+    const int64_t parts = act_parts(m, n_out, kVec<T>);
     p.rows_per_part = (m + parts - 1) / parts;
     const int64_t cols = kActLanes * kVec<T>;
     const dim3 grid(static_cast<unsigned>((n_out + cols - 1) / cols), static_cast<unsigned>(parts));

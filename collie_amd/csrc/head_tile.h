@@ -20,7 +20,10 @@
 
 namespace collie {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
@@ -34,12 +37,18 @@ __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds)
                : "memory", "m0");
 }
+// the same from a base that is the same for the wave and a lane's byte offset
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(off), "s"(lds),
+               "s"(base)
+               : "memory", "m0");
+}
 __device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-constexpr int kMfma = 0x008, kDsRead = 0x100;  // groups of __builtin_amdgcn_sched_group_barrier
+constexpr int kValu = 0x002, kMfma = 0x008, kDsRead = 0x100;  // groups of __builtin_amdgcn_sched_group_barrier
 
 // A fragment: 16 rows by 32 k; lane l holds row l % 16 and k = 8 (l / 16) + j.
 template <typename T>
@@ -61,17 +70,32 @@ struct Frag<float> {
 struct Split {
   bf16x8 hi, mid, lo;
 };
+__device__ __forceinline__ uint32_t round_pair(const f32x2& x) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+}
+__device__ __forceinline__ float low_value(uint32_t pair) {
+  return __builtin_bit_cast(float, pair << 16);
+}
+__device__ __forceinline__ float high_value(uint32_t pair) {
+  return __builtin_bit_cast(float, pair & 0xffff0000u);
+}
 template <typename T>
 __device__ __forceinline__ Split split(const Frag<T>& f) {
   Split s;
   if constexpr (sizeof(T) == 4) {
+    // two values per conversion: 44 instructions
+    u32x4 hi, mid, lo;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s.hi[j] = static_cast<bf16_t>(f.v[j]);
-      const float r = f.v[j] - static_cast<float>(s.hi[j]);
-      s.mid[j] = static_cast<bf16_t>(r);
-      s.lo[j] = static_cast<bf16_t>(r - static_cast<float>(s.mid[j]));
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 x = {f.v[2 * j], f.v[2 * j + 1]};
+      hi[j] = round_pair(x);
+      const f32x2 r = {x[0] - low_value(hi[j]), x[1] - high_value(hi[j])};
+      mid[j] = round_pair(r);
+      lo[j] = round_pair(f32x2{r[0] - low_value(mid[j]), r[1] - high_value(mid[j])});
     }
+    s.hi = __builtin_bit_cast(bf16x8, hi);
+    s.mid = __builtin_bit_cast(bf16x8, mid);
+    s.lo = __builtin_bit_cast(bf16x8, lo);
   }
   return s;
 }
@@ -160,39 +184,41 @@ struct Image {
   }
 };
 
-// The loads of one operand: every thread brings N x 16 bytes of a stage.
-//   rows0: first row of the tile; `rows` of the operand (further ones are clamped: their products go
-//   nowhere).  With SECOND, image rows from R / 2 on are rows of `p2` (the gated forward pass); with
-//   CAT, k from k_split on is k - k_split of `p2`, and of either only k < k_valid is there.
+// The loads of one operand: every thread brings N x 16 bytes of a stage, from a base that is the same
+// for the workgroup and moves by one stage, and offsets that stay.
+//   row0: first row of the tile; `rows` of the operand (further ones are clamped: their products go
+//   nowhere).  With SECOND, image rows from R / 2 on are rows of a second matrix (the gated forward
+//   pass); with CAT, k from k_split on is k - k_split of a second matrix, and of either only
+//   k < k_valid is there.
 template <typename T, int R, bool KC, int THREADS, bool SECOND, bool CAT>
 struct Feed {
   using Img = Image<T, R, KC>;
   static constexpr int N = Img::kBytes / 16 / THREADS;
   static constexpr int V = kVec<T>;
-  const T* p[N];
-  int kk[N];  // k within the stage
-  int64_t ld;
+  static constexpr int kSize = static_cast<int>(sizeof(T));
+  static_assert(!SECOND || (KC && N % 2 == 0), "the halves of an image are whole loads");
+  uint32_t off[N];            // bytes from the base: the host keeps 256 rows below 2^31
+  const char *base, *base2;   // of the next stage (base2 with CAT: at k - k_split)
+  int64_t step;
 
-  __device__ __forceinline__ void init(const void* base, const void* base2, int64_t ld_, int64_t row0,
-                                       int64_t rows, int64_t k0, int tid) {
-    ld = ld_;
+  __device__ __forceinline__ void init(const void* p, const void* p2, int64_t ld, int64_t row0,
+                                       int64_t rows, int64_t k0, int64_t k_split, int tid) {
+    const int64_t at = KC ? row0 * ld + k0 : k0 * ld + row0;
+    base = static_cast<const char*>(p) + at * kSize;
+    if (SECOND || CAT) base2 = static_cast<const char*>(p2) + (at - (CAT ? k_split * ld : 0)) * kSize;
+    step = KC ? 128 : Img::kDepth * ld * kSize;
+    const int last = static_cast<int>(rows - row0 < (SECOND ? R / 2 : R) ? rows - row0 : (SECOND ? R / 2 : R)) - 1;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       int r, c;
       Img::source(j * THREADS + tid, r, c);
       if (KC) {
-        const bool second = SECOND && r >= R / 2;
-        int64_t row = row0 + (second ? r - R / 2 : r);
-        row = row < rows ? row : rows - 1;
-        kk[j] = c * V;
-        p[j] = static_cast<const T*>(second ? base2 : base) + row * ld + k0 + kk[j];
+        if (SECOND && j >= N / 2) r -= R / 2;
+        off[j] = static_cast<uint32_t>((r < last ? r : last) * static_cast<int>(ld * kSize) + c * 16);
       } else {
         // an operand whose rows are no whole number of packs is one that was laid out with padding
-        const int64_t end = (rows + V - 1) / V * V;
-        int64_t col = row0 + c * V;
-        col = col < end ? col : end - V;
-        kk[j] = r;
-        p[j] = static_cast<const T*>(base) + col + (k0 + r) * ld;
+        off[j] = static_cast<uint32_t>(r * static_cast<int>(ld * kSize) +
+                                       (c < last / V ? c : last / V) * 16);
       }
     }
   }
@@ -200,60 +226,41 @@ struct Feed {
   // issues the loads of the stage at depth k (up to k1) into the image at LDS address `lds`
   __device__ __forceinline__ void issue(uint32_t lds, int64_t k, int64_t k1, const Gemm& g) {
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x / kWave) * kWave * 16);
-    const bool whole = k + Img::kDepth <= k1;
+    const bool second = CAT && k >= g.k_split;
+    const int64_t end = !CAT ? k1 : second ? g.k_split + g.k_valid : g.k_valid;
+    if (k + Img::kDepth <= (end < k1 ? end : k1)) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const void* q = p[j];
-      if constexpr (CAT) {
-        const int64_t at = k + kk[j];
-        const bool second = at >= g.k_split;
-        if (second) q = p[j] + g.b2_step;
-        if (!whole || g.k_valid != g.k_split) {
-          if (at >= k1 || at - (second ? g.k_split : 0) >= g.k_valid) q = &g_zero_chunk;
-        }
-      } else {
-        if (!whole && k + kk[j] >= k1) q = &g_zero_chunk;
+      for (int j = 0; j < N; ++j)
+        dma16(second || (SECOND && j >= N / 2) ? base2 : base, off[j], to + j * THREADS * 16);
+    } else {
+      // the end of the depth, or of the first matrix: lane by lane, zeros past it
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        int r, c;
+        Img::source(j * THREADS + threadIdx.x, r, c);
+        const int64_t at = k + (KC ? c * V : r);
+        const bool two = CAT ? at >= g.k_split : SECOND && j >= N / 2;
+        bool in = at < k1;
+        if (CAT) in = in && at - (two ? g.k_split : 0) < g.k_valid;
+        const char* q = (two ? base2 : base) + off[j];
+        dma16(in ? q : reinterpret_cast<const char*>(&g_zero_chunk), to + j * THREADS * 16);
       }
-      p[j] += KC ? static_cast<int64_t>(Img::kDepth) : Img::kDepth * ld;
-      dma16(q, to + j * THREADS * 16);
     }
+    base += step;
+    if (SECOND || CAT) base2 += step;
   }
 };
 
-// Lanes l, l + 16, l + 32, l + 48 hold columns 4 q .. 4 q + 3 (q = l / 16) of one row of two or four
-// 16-column tiles.  Afterwards lane row q holds, of four tiles, all of tile q; of two tiles, the half
-// q / 2 of tile q % 2.
-__device__ __forceinline__ void swap_lanes16(float& a, float& b) {
-  const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a),
-                                                  __builtin_bit_cast(uint32_t, b), false, false);
-  const uint32_t a1 = s[0], b1 = s[1];  // (a bit_cast of a vector's element would take element 0)
-  a = __builtin_bit_cast(float, a1);
-  b = __builtin_bit_cast(float, b1);
-}
-__device__ __forceinline__ void swap_lanes32(float& a, float& b) {
-  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a),
-                                                  __builtin_bit_cast(uint32_t, b), false, false);
-  const uint32_t a1 = s[0], b1 = s[1];  // (a bit_cast of a vector's element would take element 0)
-  a = __builtin_bit_cast(float, a1);
-  b = __builtin_bit_cast(float, b1);
-}
+// Lanes l, l + 16, l + 32, l + 48 hold columns 4 q .. 4 q + 3 (q = l / 16) of one row of two 16-column
+// tiles; afterwards lane row q holds half q / 2 of tile q % 2.
 __device__ __forceinline__ void spread2(const f32x4& t0, const f32x4& t1, float (&v)[8]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    v[j] = t0[j];
-    v[4 + j] = t1[j];
-    swap_lanes16(v[j], v[4 + j]);
-  }
-}
-__device__ __forceinline__ void spread4(const f32x4 (&t)[4], float (&v)[16]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[4 * k + j] = t[k][j];
-    swap_lanes32(v[j], v[8 + j]);
-    swap_lanes32(v[4 + j], v[12 + j]);
-    swap_lanes16(v[j], v[4 + j]);
-    swap_lanes16(v[8 + j], v[12 + j]);
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(t0[j]), __float_as_uint(t1[j]),
+                                                    false, false);
+    const uint32_t a = s[0], b = s[1];  // (a bit_cast of a vector's element would take element 0)
+    v[j] = __uint_as_float(a);
+    v[4 + j] = __uint_as_float(b);
   }
 }
 
@@ -275,6 +282,9 @@ __device__ __forceinline__ void tile_at(int64_t id, int64_t tiles_m, int64_t til
   tn = id / high;
 }
 
+// The grid is at most what the chip holds: a workgroup works on one tile (or one part of the depth of
+// a tile) after another, and the first stage of the next one is loaded under the last products and
+// the epilogue of the one before.
 template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool CAT>
 __global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm g) {
   constexpr bool PAIR = EPI == kEpiGated;
@@ -294,138 +304,211 @@ __global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm 
   const int wm = wave / WN, wn = wave % WN;
 
   const int64_t tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + TN - 1) / TN;
-  const bool cut = blockIdx.x >= g.full;  // one part of the depth of a tile
-  int64_t id, part = 0, tm, tn;
-  if (cut) {
-    const int64_t rest = tiles_m * tiles_n - g.full;
-    id = xcd_order(blockIdx.x - g.full, rest * g.splits);
-    part = id / rest;
-    id = g.full + id % rest;
-  } else {
-    id = xcd_order(blockIdx.x, g.full);
-  }
-  tile_at(id, tiles_m, tiles_n, tm, tn);
-  const int64_t row0 = tm * BM, col0 = tn * TN;
-  const int64_t k0 = cut ? part * g.k_chunk : 0;
-  const int64_t k1 = cut && k0 + g.k_chunk < g.k ? k0 + g.k_chunk : g.k;
+  const int64_t rest = tiles_m * tiles_n - g.full;
+  const int64_t total = g.full + rest * g.splits;
+  struct Work {
+    int64_t slot, row0, col0, k0, k1;  // slot: of the partial sums, -1 for a whole tile
+  };
+  auto work_at = [&](int64_t n) {
+    Work w;
+    int64_t id, tm, tn;
+    if (n >= g.full) {
+      id = xcd_order(n - g.full, rest * g.splits);
+      w.slot = id;
+      w.k0 = id / rest * g.k_chunk;
+      w.k1 = w.k0 + g.k_chunk < g.k ? w.k0 + g.k_chunk : g.k;
+      id = g.full + id % rest;
+    } else {
+      id = xcd_order(n, g.full);
+      w.slot = -1;
+      w.k0 = 0;
+      w.k1 = g.k;
+    }
+    tile_at(id, tiles_m, tiles_n, tm, tn);
+    w.row0 = tm * BM;
+    w.col0 = tn * TN;
+    return w;
+  };
 
+  Feed<T, BM, AKC, THREADS, false, false> fa;
+  Feed<T, BN, BKC, THREADS, PAIR, CAT> fb;
+  auto start = [&](const Work& w, uint32_t to) {
+    fa.init(g.a.p, nullptr, AKC ? g.a.rs : g.a.ks, w.row0, g.m, w.k0, 0, tid);
+    fb.init(g.b.p, g.b2, BKC ? g.b.rs : g.b.ks, w.col0, g.n, w.k0, g.k_split, tid);
+    fa.issue(to, w.k0, w.k1, g);
+    fb.issue(to + ImgA::kBytes, w.k0, w.k1, g);
+  };
   f32x4 acc[MT][NT];
+  auto b_row = [&](int j) {
+    return PAIR ? (j / HALF) * (BN / 2) + wn * (TN / WN) + (j % HALF) * 16 : wn * (BN / WN) + j * 16;
+  };
   // float32: EXACT takes the float32 instructions
-  auto product = [&](auto exact) {
+  auto products = [&](const char* ia, auto exact) {
     constexpr bool EXACT = decltype(exact)::value;
-    Feed<T, BM, AKC, THREADS, false, false> fa;
-    Feed<T, BN, BKC, THREADS, PAIR, CAT> fb;
-    fa.init(g.a.p, nullptr, AKC ? g.a.rs : g.a.ks, row0, g.m, k0, tid);
-    fb.init(g.b.p, g.b2, BKC ? g.b.rs : g.b.ks, col0, g.n, k0, tid);
+    const char* ib = ia + ImgA::kBytes;
+    if constexpr (sizeof(T) == 4 && !EXACT) {
+      constexpr int RA32 = AKC ? 2 : 8, RB32 = BKC ? 2 : 8;
+      Split b[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) b[j] = split(ImgB::read(ib, b_row(j), 0, lane));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const Split a = split(ImgA::read(ia, wm * (BM / WM) + i * 16, 0, lane));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) multiply(b[j], a, acc[i][j]);
+      }
+      // the split of the next row tile goes between the products of this one
+      __builtin_amdgcn_sched_group_barrier(kDsRead, RA32 + RB32 * NT, 0);
+      __builtin_amdgcn_sched_group_barrier(kValu, 46 * (NT + 1), 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, RA32, 0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int t = 0; t < 6 * NT; ++t) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kValu, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kDsRead, RA32, 0);
+      }
+    } else {
+#pragma unroll
+      for (int step = 0; step < ImgA::kSteps; ++step) {
+        Frag<T> b[NT], a[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) b[j] = ImgB::read(ib, b_row(j), step, lane);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[i] = ImgA::read(ia, wm * (BM / WM) + i * 16, step, lane);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) multiply<T>(b[j], a[i], acc[i][j]);
+      }
+      if constexpr (sizeof(T) == 2) {
+        // the order of the above: the fragments of the next row tiles are on their way while those at
+        // hand are multiplied (8,192^3: 1,025 -> 990 us)
+        constexpr int RA = AKC ? 1 : 2, RB = BKC ? 1 : 2;  // LDS reads per fragment
+        __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB + 2 * RA, 0);
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+#pragma unroll
+          for (int i = 0; i < MT - 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, RA, 0);
+          }
+          if (step == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+              __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB / 2 + RA, 0);
+            }
+          } else {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 2 * NT, 0);
+          }
+        }
+      }
+    }
+  };
+  auto clear = [&] {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    fa.issue(lds0, k0, k1, g);
-    fb.issue(lds0 + ImgA::kBytes, k0, k1, g);
-    int cur = 0;
-    for (int64_t k = k0; k < k1; k += kDepth) {
-      wait_dma();      // this wave's loads of the stage have landed
-      tile_barrier();  // everyone's have, and the other stage has been read
-      if (k + kDepth < k1) {
-        const uint32_t to = lds0 + (cur ^ 1) * kStage;
-        fa.issue(to, k + kDepth, k1, g);
-        fb.issue(to + ImgA::kBytes, k + kDepth, k1, g);
-      }
-      const char* ia = lds + cur * kStage;
-      const char* ib = ia + ImgA::kBytes;
-      auto b_row = [&](int j) {
-        return PAIR ? (j / HALF) * (BN / 2) + wn * (TN / WN) + (j % HALF) * 16
-                    : wn * (BN / WN) + j * 16;
-      };
-      if constexpr (sizeof(T) == 4 && !EXACT) {
-        Split b[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) b[j] = split(ImgB::read(ib, b_row(j), 0, lane));
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const Split a = split(ImgA::read(ia, wm * (BM / WM) + i * 16, 0, lane));
-#pragma unroll
-          for (int j = 0; j < NT; ++j) multiply(b[j], a, acc[i][j]);
-        }
-      } else {
-#pragma unroll
-        for (int step = 0; step < ImgA::kSteps; ++step) {
-          Frag<T> b[NT], a[MT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) b[j] = ImgB::read(ib, b_row(j), step, lane);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) a[i] = ImgA::read(ia, wm * (BM / WM) + i * 16, step, lane);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) multiply<T>(b[j], a[i], acc[i][j]);
-        }
-        if constexpr (sizeof(T) == 2) {
-          // the order of the above: the fragments of the next row tiles are on their way while those
-          // at hand are multiplied
-          constexpr int RA = AKC ? 1 : 2, RB = BKC ? 1 : 2;  // LDS reads per fragment
-          __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB + 2 * RA, 0);
-#pragma unroll
-          for (int step = 0; step < 2; ++step) {
-#pragma unroll
-            for (int i = 0; i < MT - 2; ++i) {
-              __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
-              __builtin_amdgcn_sched_group_barrier(kDsRead, RA, 0);
-            }
-            if (step == 0) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
-                __builtin_amdgcn_sched_group_barrier(kDsRead, NT * RB / 2 + RA, 0);
-              }
-            } else {
-              __builtin_amdgcn_sched_group_barrier(kMfma, 2 * NT, 0);
-            }
-          }
-        }
-      }
-      cur ^= 1;
-    }
   };
-  product(std::false_type{});
-  if constexpr (sizeof(T) == 4) {
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) finite = finite && fabsf(acc[i][j][t]) < INFINITY;
-    if (__syncthreads_or(!finite)) product(std::true_type{});
-  }
 
-  // Four neighbouring columns per lane would be stored as pieces of 8 bytes.  The lanes that hold a
-  // row exchange theirs, so that one has W neighbouring columns and a row leaves in whole lines.
   static_assert(NT == 4, "four column tiles per wave");
-  constexpr int W = PAIR ? 8 : 16;
-  const int r = lane & 15, q = lane >> 4;
-  const int lc = PAIR ? wn * (TN / WN) + 16 * (q & 1) + 8 * (q >> 1) : wn * (TN / WN) + 16 * q;
-  float b[W], b2[W];
-  if (!cut) load_biases<T, EPI, W>(g, col0 + lc, b, b2);
+  constexpr int W = sizeof(T) == 4 ? 4 : 8;  // columns that a lane stores together
+  constexpr int G = 4 * HALF / W;
+
+  int64_t n = blockIdx.x;
+  Work now = work_at(n);
+  int cur = 0;
+  start(now, lds0);
+  while (true) {
+    const bool more = n + gridDim.x < total;
+    const Work next = more ? work_at(n + gridDim.x) : now;
+    clear();
+    wait_dma();  // this wave's loads of the first stage have landed (so they have further down)
+    for (int64_t k = now.k0; k < now.k1; k += kDepth) {
+      tile_barrier();  // every wave's loads have landed, and the other stage has been read
+      const uint32_t to = lds0 + (cur ^ 1) * kStage;
+      if (k + kDepth < now.k1) {
+        fa.issue(to, k + kDepth, now.k1, g);
+        fb.issue(to + ImgA::kBytes, k + kDepth, now.k1, g);
+      } else if (more) {
+        start(next, to);
+      }
+      products(lds + cur * kStage, std::false_type{});
+      cur ^= 1;
+      if (k + kDepth < now.k1) wait_dma();
+    }
+    if constexpr (sizeof(T) == 4) {
+      bool finite = true;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int lr = wm * (BM / WM) + i * 16 + r;
-    float v[W], u[W];
-    if constexpr (PAIR) {
-      spread2(acc[i][0], acc[i][1], v);
-      spread2(acc[i][2], acc[i][3], u);
-    } else {
-      spread4(acc[i], v);
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) finite = finite && fabsf(acc[i][j][t]) < INFINITY;
+      if (__syncthreads_or(!finite)) {
+        // once more, one stage at a time in the stage that holds nothing, then the next tile's first
+        // stage again (the loads above went on from there)
+        clear();
+        const uint32_t to = lds0 + (cur ^ 1) * kStage;
+        for (int64_t k = now.k0; k < now.k1; k += kDepth) {
+          wait_dma();
+          tile_barrier();
+          if (k == now.k0) {
+            start(now, to);
+          } else {
+            fa.issue(to, k, now.k1, g);
+            fb.issue(to + ImgA::kBytes, k, now.k1, g);
+          }
+          wait_dma();
+          tile_barrier();
+          products(lds + (cur ^ 1) * kStage, std::true_type{});
+        }
+        tile_barrier();
+        if (more) start(next, lds0 + cur * kStage);
+      }
     }
-    if (cut) {
-      const int64_t rest = tiles_m * tiles_n - g.full;
-      float* p = g.partial + ((part * rest + id - g.full) * (PAIR ? 2 : 1) * BM + lr) * TN + lc;
-      store_pack<float, W>(p, W, v);
-      if (PAIR) store_pack<float, W>(p + BM * TN, W, u);
-    } else {
-      finish_row<T, EPI, W>(g, row0 + lr, col0 + lc, v, u, b, b2);
+
+    // A lane has four neighbouring columns of each column tile.  Of float32, four lanes then store a
+    // 64-byte piece of a row; of 16 bits, lanes exchange halves of two tiles to the same end.
+    const int r = lane & 15, q = lane >> 4;
+    const int lc0 = wn * (TN / WN) + (W == 4 ? 4 * q : 16 * (q & 1) + 8 * (q >> 1));
+    float b[G][W], b2[G][W];
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (now.slot < 0) load_biases<T, EPI, W>(g, now.col0 + lc0 + k * 4 * W, b[k], b2[k]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int lr = wm * (BM / WM) + i * 16 + r;
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        const int lc = lc0 + k * 4 * W;
+        float v[W], u[W];
+        if constexpr (W == 4) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            v[t] = acc[i][k][t];
+            u[t] = acc[i][PAIR ? k + HALF : k][t];
+          }
+        } else {
+          spread2(acc[i][2 * k], acc[i][2 * k + 1], v);
+          if constexpr (PAIR) spread2(acc[i][2], acc[i][3], u);
+        }
+        if (now.slot >= 0) {
+          float* p = g.partial + (now.slot * (PAIR ? 2 : 1) * BM + lr) * TN + lc;
+          store_pack<float, W>(p, W, v);
+          if (PAIR) store_pack<float, W>(p + BM * TN, W, u);
+        } else {
+          finish_row<T, EPI, W>(g, now.row0 + lr, now.col0 + lc, v, u, b[k], b2[k]);
+        }
+      }
     }
+    if (!more) break;
+    n += gridDim.x;
+    now = next;
   }
 }
 
