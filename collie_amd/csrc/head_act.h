@@ -21,6 +21,22 @@ __device__ __forceinline__ float fast_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z));
 }
 
+// Phi(z), the normal distribution function, and exp(-z^2 / 2) with it: Abramowitz and Stegun, Handbook
+// of Mathematical Functions, 7.1.26 (erfc to 1.5e-7), without a branch; the side of small values is
+// computed as such.  The library's erff cost the forward pass of 720,896 x 256 x 128 (float32) 100 us
+// of 580.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+  float p = fmaf(t, 1.061405429f, -1.453152027f);
+  p = fmaf(t, p, 1.421413741f);
+  p = fmaf(t, p, -0.284496736f);
+  p = fmaf(t, p, 0.254829592f);
+  e = fast_exp(-x * x);
+  const float tail = 0.5f * p * t * e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
 // f(z) over N values; `act` is the same for the whole launch, so the branch is taken once
 template <int N>
 __device__ __forceinline__ void act_values(int act, float (&v)[N]) {
@@ -43,7 +59,10 @@ __device__ __forceinline__ void act_values(int act, float (&v)[N]) {
       break;
     case COLLIE_ACT_GELU:
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] * (0.5f * (1.0f + erff(v[i] * 0.70710678118654752f)));
+      for (int i = 0; i < N; ++i) {
+        float e;
+        v[i] *= normal_cdf(v[i], e);
+      }
       break;
     default: break;
   }
@@ -85,8 +104,9 @@ __device__ __forceinline__ void act_slopes(int act, float (&v)[N], float (&d)[N]
     case COLLIE_ACT_GELU:
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float cdf = 0.5f * (1.0f + erff(v[i] * 0.70710678118654752f));
-        d[i] = cdf + v[i] * (0.39894228040143268f * fast_exp(-0.5f * v[i] * v[i]));
+        float e;
+        const float cdf = normal_cdf(v[i], e);
+        d[i] = fmaf(v[i] * 0.39894228f, e, cdf);
         v[i] *= cdf;
       }
       break;

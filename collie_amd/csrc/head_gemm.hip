@@ -267,12 +267,12 @@ int launch_skinny(const Gemm& g, hipStream_t stream) {
   return -1;
 }
 
-// slices of the rows for the column sums: together with the column blocks about sixteen workgroups per
+// slices of the rows for the column sums: together with the column blocks about eight workgroups per
 // CU (with two, 720,896 x 128 float32 ran at 2.8 of the 4.7 TB/s a copy reaches), each of at least
 // four rows per lane group
 int64_t act_parts(int64_t m, int64_t n, int64_t v) {
   const int64_t columns = (n + kActLanes * v - 1) / (kActLanes * v);
-  int64_t parts = (4096 + columns - 1) / columns;
+  int64_t parts = (2048 + columns - 1) / columns;
   if (parts < 64) parts = 64;
   const int64_t most = (m + 4 * kActRows - 1) / (4 * kActRows);
   return parts < most ? parts : most;

@@ -30,6 +30,7 @@ struct NormParams {
   int dim;
   int w_f32;         // w and b are float32 (else: the rows' type)
   float eps;
+  bool stream;       // the result is stored past the caches
 };
 
 template <typename T, int V>
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_kernel(const NormParams p) {
     const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.x_ld;
     float v[NV][V], s[1] = {0.0f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_row<WHOLE, T, V>(x + col[i], left[i], left[i] > 0, v[i]);
+    for (int i = 0; i < NV; ++i) load_row<WHOLE, T, V>(x, col[i], p.dim, left[i] > 0, v[i]);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_kernel(const NormParams p) {
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
-      if (left[i] > 0) store_pack<T, V>(y + col[i], left[i], v[i]);
+      if (left[i] > 0) store_pack<T, V>(y + col[i], left[i], v[i], p.stream);
     }
     if (sub == 0 && p.mean) {
       p.mean[row] = mean;
@@ -150,8 +151,8 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const NormParams p) {
     float h[NV][V], g[NV][V], s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      load_row<WHOLE, T, V>(x + col[i], left[i], left[i] > 0, h[i]);
-      load_row<WHOLE, T, V>(dy + col[i], left[i], left[i] > 0 && live, g[i]);
+      load_row<WHOLE, T, V>(x, col[i], p.dim, left[i] > 0, h[i]);
+      load_row<WHOLE, T, V>(dy, col[i], p.dim, left[i] > 0 && live, g[i]);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const NormParams p) {
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) g[i][j] = rstd * (g[i][j] - fmaf(h[i][j], mgh, mg));
-      if (left[i] > 0) store_pack<T, V>(dx + col[i], left[i], g[i]);
+      if (left[i] > 0) store_pack<T, V>(dx + col[i], left[i], g[i], p.stream);
     }
   }
   if (p.partial == nullptr) return;
@@ -434,6 +435,7 @@ extern "C" int collie_layer_norm_forward(const void* x, int64_t x_ld, int32_t dt
     p.dim = dim;
     p.w_f32 = w_dtype == COLLIE_F32;
     p.eps = eps;
+    p.stream = rows * dim * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
     const NormShape s = norm_shape<T>(dim);
     const int64_t groups = s.tpr ? kBlock / s.tpr : 1;
     int64_t grid = (rows + groups - 1) / groups;
@@ -483,6 +485,7 @@ extern "C" int collie_layer_norm_backward(const void* dy, int64_t dy_ld, const v
     p.dy_ld = dy_ld;
     p.dim = dim;
     p.w_f32 = w_dtype == COLLIE_F32;
+    p.stream = rows * dim * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
     const int count = rows ? norm_partials<T>(rows, dim) : 0;
     const NormShape s = norm_shape<T>(dim);
     if (rows && s.tpr && (dx || sums)) {
