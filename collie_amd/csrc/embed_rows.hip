@@ -20,9 +20,10 @@ constexpr int kLookupRows = 4;                 // rows in flight per lane group 
 constexpr int kAhead = 8;                      // rows on their way while as many are summed
 constexpr uint32_t kNoKey = 0xffffffffu;       // no entry (keys are rows, below 2^31)
 
-// `lpr` lanes per row, a power of two: at most a wave, and no more than the row has 16-byte chunks
-inline int lanes_per_row(int64_t dim, int v) {
-  int l = 1;
+// `lpr` lanes per row, a power of two: at most a wave, and no more than the row has 16-byte packs, but
+// at least `least`
+inline int lanes_per_row(int64_t dim, int v, int least) {
+  int l = least;
   while (l < kWave && static_cast<int64_t>(l) * v < dim) l <<= 1;
   return l;
 }
@@ -77,8 +78,11 @@ __global__ __launch_bounds__(kBlock) void grad_entries_kernel(
     keys[i] = static_cast<uint32_t>(ok && id != padding_idx ? id : num_rows);
     codes[i] = static_cast<uint32_t>(i);
   }
+  // a workgroup fills one contiguous piece (512 MB: 6 TB/s; round-robin 16-byte stores 3.7)
   const int64_t n16 = grad_bytes / 16;
-  for (int64_t i = t0; i < n16; i += stride)
+  const int64_t piece = (n16 + gridDim.x - 1) / gridDim.x;
+  const int64_t end = (blockIdx.x + 1) * piece < n16 ? (blockIdx.x + 1) * piece : n16;
+  for (int64_t i = blockIdx.x * piece + threadIdx.x; i < end; i += kBlock)
     reinterpret_cast<uint4*>(grad)[i] = make_uint4(0, 0, 0, 0);
   for (int64_t i = 8 * n16 + t0; i < grad_bytes / 2; i += stride)
     reinterpret_cast<uint16_t*>(grad)[i] = 0;
@@ -232,7 +236,9 @@ struct RunShape {
 };
 RunShape run_shape(int64_t m, int dim, int v, bool later) {
   RunShape r;
-  r.lpr = lanes_per_row(dim, v);
+  // eight lanes also where fewer would do: of a run that fills the workgroup one lane group adds up the
+  // open sums of all, and there are 32 of them then, not 256 (1 column, 65,536 skewed ids: 105 -> 55 us)
+  r.lpr = lanes_per_row(dim, v, 8);
   const int groups = kBlock / r.lpr;
   const int most = kMaxEntries / groups < kMaxChunk ? kMaxEntries / groups : kMaxChunk;
   r.chunk = most;
@@ -306,7 +312,7 @@ extern "C" int collie_embedding_rows(const void* table, int32_t dtype, int64_t n
   COLLIE_REQUIRE(table && ids && out, "embedding_rows: NULL pointer");
   return with_type(dtype, "embedding_rows", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    const int lpr = lanes_per_row(dim, kVec<T>);
+    const int lpr = lanes_per_row(dim, kVec<T>, 1);
     const int64_t per_block = static_cast<int64_t>(kBlock / lpr) * kLookupRows;
     auto* kernel = dim % kVec<T> == 0 ? embed_rows_kernel<T, true> : embed_rows_kernel<T, false>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + per_block - 1) / per_block)),

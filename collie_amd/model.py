@@ -29,7 +29,7 @@ import torch
 from torch import nn
 from torch.optim.lr_scheduler import ReduceLROnPlateau
 
-from collie_amd import _lib, loss as loss_mod, ops
+from collie_amd import _lib, functional, loss as loss_mod, ops
 from collie_amd.interactions import (ApproximateNegativeSamplingInteractionsDataLoader,
                                      Interactions, InteractionsDataLoader)
 from collie_amd.layers import ScaledEmbedding, ZeroEmbedding
@@ -65,16 +65,13 @@ class _MFScore(torch.autograd.Function):
         tables = _lib.make_tables(ue, ie, ub, ib)
         gu, gi, gb = ops.mf_score_backward(tables, users, items, grad_out, ctx.y_range, ctx.status,
                                            ctx.dropout)
-        u_idx = users.long().reshape(1, -1)
-        i_idx = items.long().reshape(1, -1)
-
-        def build(idx, vals, like):
+        def build(ids, vals, like):
             if ctx.sparse:      # the uncoalesced COO gradient nn.Embedding(sparse=True) produces
-                return torch.sparse_coo_tensor(idx, vals, like.shape)
-            return torch.zeros_like(like).index_add_(0, idx[0], vals)
+                return torch.sparse_coo_tensor(ids.long().reshape(1, -1), vals, like.shape)
+            return functional.table_grad(like, ids, vals, ctx.status)
 
-        return (None, None, build(u_idx, gu, ue), build(i_idx, gi, ie), build(u_idx, gb, ub),
-                build(i_idx, gb, ib), None, None, None, None)
+        return (None, None, build(users, gu, ue), build(items, gi, ie), build(users, gb, ub),
+                build(items, gb, ib), None, None, None, None)
 
 
 # ---- fused route: calculate_loss ---------------------------------------------------------------

@@ -3,6 +3,7 @@ Thin tensor-level wrappers over the C ABI: they only marshal torch tensors (devi
 current HIP stream) into ``libcollie_hip.so`` calls.  No arithmetic happens in this file.
 """
 import ctypes
+import functools
 from ctypes import byref, c_void_p
 
 import torch
@@ -970,9 +971,16 @@ def rows_view(t, width):
     return t, (t.stride(0) if t.shape[0] > 1 else width)
 
 
-def _workspace(need, like):
+@functools.lru_cache(maxsize=4096)
+def _bytes(name, *args):
+    """Workspace size ``name(*args)``.  Of addresses only the alignment counts: callers pass their
+    last four bits."""
+    return getattr(load(), name)(*args)
+
+
+def _workspace(like, name, *args):
     """Scratch of one call (its caller holds it until the launches are in the stream)."""
-    return torch.empty(need, dtype=torch.uint8, device=like.device)
+    return torch.empty(_bytes(name, *args), dtype=torch.uint8, device=like.device)
 
 
 def embedding_rows(table, ids, scale=1.0, status=None):
@@ -1007,7 +1015,7 @@ def embedding_rows_grad(ids, dy, num_rows, scale=1.0, padding_idx=None, status=N
     ids = ids.contiguous()
     dy, ld = rows_view(dy, dim)
     grad = torch.empty((num_rows, dim), dtype=dy.dtype, device=dy.device)
-    ws = _workspace(load().collie_embedding_rows_grad_workspace_bytes(n, dim), dy)
+    ws = _workspace(dy, 'collie_embedding_rows_grad_workspace_bytes', n, dim)
     _call(dy, 'collie_embedding_rows_grad', ids.data_ptr(), idx_dtype(ids), n, dy.data_ptr(), ld, tag,
           num_rows, dim, scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(),
           ws.data_ptr(), ws.numel(), _at(status))
@@ -1065,7 +1073,7 @@ def layer_norm_backward(dy, x, weight, bias, stats, want):
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
     dw, db = (torch.empty((dim,), dtype=p.dtype, device=x.device) if w and p is not None else None
               for w, p in zip(want[1:], (weight, bias)))
-    ws = _workspace(load().collie_layer_norm_backward_workspace_bytes(m, dim), x)
+    ws = _workspace(x, 'collie_layer_norm_backward_workspace_bytes', m, dim)
     _call(x, 'collie_layer_norm_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, dim,
           _at(weight.contiguous() if weight is not None else None),
           _norm_param_tag(weight, bias, tag), stats.data_ptr(), stats.data_ptr() + 4 * m, _at(dx),
@@ -1119,8 +1127,8 @@ def linear_forward(x, weight, bias, activation, residual, keep):
         res, res_ld = rows_view(_param_rows(residual, x, shape, 'residual'), n_out)
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     kept = torch.empty((m, n_out), dtype=x.dtype, device=x.device) if keep and act else None
-    ws = _workspace(load().collie_layer_forward_workspace_bytes(
-        rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), None, n_out), x)
+    ws = _workspace(x, 'collie_layer_forward_workspace_bytes', rows.data_ptr() & 15, ld, tag, m, n_in,
+                    weight.data_ptr() & 15, None, n_out)
     _call(x, 'collie_linear_forward', rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), _at(bias),
           n_out, act, _at(res), res_ld, _at(kept), y.data_ptr(), ws.data_ptr(), ws.numel())
     return y, kept
@@ -1140,9 +1148,8 @@ def linear_backward(dy, x, weight, activation, kept, want):
     weight = weight.contiguous()
     dy, dy_ld = rows_view(dy, n_out)
     tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
-    ws = _workspace(load().collie_layer_backward_workspace_bytes(
-        dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), None, n_out,
-        act), x)
+    ws = _workspace(x, 'collie_layer_backward_workspace_bytes', dy.data_ptr() & 15, dy_ld,
+                    rows.data_ptr() & 15, ld, tag, m, n_in, weight.data_ptr() & 15, None, n_out, act)
     _call(x, 'collie_linear_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
           weight.data_ptr(), n_out, act, _at(kept), _at(dx), _at(dw), _at(db),
           ws.data_ptr(), ws.numel())
@@ -1161,8 +1168,8 @@ def gated_forward(x, gate_weight, up_weight, gate_bias, up_bias, activation, kee
     g = u = None
     if keep:
         g, u = torch.empty((2, m, n_out), dtype=torch.float32, device=x.device)
-    ws = _workspace(load().collie_layer_forward_workspace_bytes(
-        rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(), n_out), x)
+    ws = _workspace(x, 'collie_layer_forward_workspace_bytes', rows.data_ptr() & 15, ld, tag, m, n_in,
+                    wg.data_ptr() & 15, 16 | wu.data_ptr() & 15, n_out)
     _call(x, 'collie_gated_forward', rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(),
           _at(bg), _at(bu), n_out, act, _at(g), _at(u), y.data_ptr(), ws.data_ptr(), ws.numel())
     return y, g, u
@@ -1182,9 +1189,9 @@ def gated_backward(dy, x, gate_weight, up_weight, activation, kept_gate, kept_up
     wg, wu = gate_weight.contiguous(), up_weight.contiguous()
     dy, dy_ld = rows_view(dy, n_out)
     tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
-    ws = _workspace(load().collie_layer_backward_workspace_bytes(
-        dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(), n_out,
-        act), x)
+    ws = _workspace(x, 'collie_layer_backward_workspace_bytes', dy.data_ptr() & 15, dy_ld,
+                    rows.data_ptr() & 15, ld, tag, m, n_in, wg.data_ptr() & 15,
+                    16 | wu.data_ptr() & 15, n_out, act)
     _call(x, 'collie_gated_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
           wg.data_ptr(), wu.data_ptr(), n_out, act, kept_gate.data_ptr(), kept_up.data_ptr(),
           *[_at(t) for t in out], ws.data_ptr(), ws.numel())

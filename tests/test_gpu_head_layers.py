@@ -141,6 +141,48 @@ def test_table_modules_give_what_torch_gives(cls, sparse):
     assert torch.equal((t.weight.grad.to_dense() if sparse else t.weight.grad).cpu(), want)
 
 
+@pytest.mark.parametrize('n', [0, 1000, 70000])
+@pytest.mark.parametrize('dim', [1, 24])
+def test_dense_table_gradients_of_the_models(n, dim):
+    """Few rows by atomic adds, many by sorted ids: the same sums."""
+    from collie_amd import functional as F
+    assert n < F.SORTED_GRAD_ROWS or n > F.SORTED_GRAD_ROWS
+    ids, vals = make_ids(500, n, 'skew', 3).int(), rand((n, dim), torch.float32, 4)
+    table = torch.zeros(500, dim, device=DEV)
+    got = F.table_grad(table, ids.to(DEV), vals.to(DEV))
+    want = torch.zeros(500, dim, dtype=torch.float64).index_add_(0, ids, vals.double())
+    mag = torch.zeros(500, dim, dtype=torch.float64).index_add_(0, ids, vals.double().abs())
+    hb.check(got, want, (torch.bincount(ids, minlength=500)[:, None] + 2) * hb.F * mag,
+             torch.float32)
+
+
+def test_generic_route_of_a_dense_model_on_a_large_batch():
+    from collie_amd.model import MatrixFactorizationModel
+
+    class Shape:
+        num_users, num_items, num_negative_samples = 300, 200, 1
+
+    torch.manual_seed(0)
+    model = MatrixFactorizationModel(train=Shape(), embedding_dim=16, sparse=False,
+                                     lr_scheduler_func=None).to(DEV)
+    with torch.no_grad():
+        for t in (model.user_embeddings, model.item_embeddings):
+            t.weight.copy_(torch.randn(t.weight.shape))
+    users, items = make_ids(300, 70000, 'skew', 5), make_ids(200, 70000, 'skew', 6)
+    c = rand((70000,), torch.float32, 7)
+    (model(users.to(DEV), items.to(DEV)) * c.to(DEV)).sum().backward()
+    rows = {'user_embeddings': (users, model.item_embeddings.weight.detach().cpu()[items]),
+            'item_embeddings': (items, model.user_embeddings.weight.detach().cpu()[users]),
+            'user_biases': (users, torch.ones(70000, 1)), 'item_biases': (items, torch.ones(70000, 1))}
+    for name, (ids, other) in rows.items():
+        table = getattr(model, name).weight
+        vals = c.double()[:, None] * other.double()
+        want = torch.zeros(table.shape, dtype=torch.float64).index_add_(0, ids, vals)
+        mag = torch.zeros(table.shape, dtype=torch.float64).index_add_(0, ids, vals.abs())
+        count = torch.bincount(ids, minlength=table.shape[0])[:, None]
+        hb.check(table.grad, want, (count + 4) * hb.F * mag, torch.float32)
+
+
 # ---- layer norm ----------------------------------------------------------------------------------
 NORM = [(1, 1), (1, 128), (3, 5), (17, 64), (130, 65), (64, 128), (33, 255), (9, 256), (70, 511),
         (20, 1000), (40, 1023), (5, 1025), (6, 2048), (11, 3001), (4, 4096), (3, 8191), (2, 8192),
