@@ -28,7 +28,7 @@ from torch import nn
 from torch.optim.lr_scheduler import ReduceLROnPlateau
 
 from collie_amd import _lib, functional, ops
-from collie_amd.layers import ScaledEmbedding, ZeroEmbedding
+from collie_amd.layers import GatedLinear, LayerNorm, Linear, ScaledEmbedding, ZeroEmbedding
 from collie_amd.model import INTERACTIONS_LIKE_INPUT, MatrixFactorizationModel
 from collie_amd.optim import FusedAdagrad, FusedAdam, FusedSGD
 
@@ -141,8 +141,13 @@ class HybridPretrainedModel(MatrixFactorizationModel):
     Parameters are those of the reference (``hybrid_pretrained_matrix_factorization.py:102-126``):
     ``train, val, item_metadata, user_metadata, trained_model, item_metadata_layers_dims,
     user_metadata_layers_dims, combined_layers_dims=[128, 64, 32], freeze_embeddings=True,
-    dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', loss='hinge',
+dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', loss='hinge',
     metadata_for_loss, metadata_for_loss_weights, load_model_path, map_location``.
+
+    One more, ``combined_blocks`` (0: the reference's head), makes the head deeper: that many residual
+    blocks ``h + back(gated(norm(h)))`` (``layers.LayerNorm`` / ``GatedLinear`` with twice the width /
+    ``Linear``, named ``combined_block_<i>``) between the first combined layer and the others.  Such a
+    head runs on ``collie_amd.functional`` and autograd.
     """
     _mf_eval_fast = False       # evaluation goes through get_preds (the score is not a dot product)
     _active_rows_hint = None    # see calculate_loss / _head_backward
@@ -174,8 +179,11 @@ class HybridPretrainedModel(MatrixFactorizationModel):
                  metadata_for_loss: Optional[Dict[str, torch.Tensor]] = None,
                  metadata_for_loss_weights: Optional[Dict[str, float]] = None,
                  load_model_path: Optional[str] = None,
-                 map_location: Optional[str] = None):
+                 map_location: Optional[str] = None,
+                 combined_blocks: int = 0):
         item_cols = user_cols = None
+        if combined_blocks < 0:
+            raise ValueError(f'combined_blocks must not be negative, not {combined_blocks}')
         if load_model_path is None:
             if trained_model is None:
                 raise ValueError('Must provide ``trained_model`` for ``HybridPretrainedModel``.')
@@ -191,6 +199,7 @@ class HybridPretrainedModel(MatrixFactorizationModel):
             hp=dict(item_metadata_layers_dims=item_metadata_layers_dims,
                     user_metadata_layers_dims=user_metadata_layers_dims,
                     combined_layers_dims=list(combined_layers_dims),
+                    combined_blocks=int(combined_blocks),
                     freeze_embeddings=freeze_embeddings, item_metadata_num_cols=item_cols,
                     user_metadata_num_cols=user_cols))
         self.item_metadata = None
@@ -270,6 +279,18 @@ class HybridPretrainedModel(MatrixFactorizationModel):
         for i, layer in enumerate(self.combined_layers):
             nn.init.xavier_normal_(layer.weight)
             self.add_module('combined_layer_{}'.format(i), layer)
+        # (hyper-parameters saved before there were blocks do not name them)
+        self.combined_blocks = []
+        for i in range(hp.get('combined_blocks') or 0):
+            if len(self.combined_layers) < 2:
+                raise ValueError('combined_blocks need at least one entry in combined_layers_dims')
+            block = nn.ModuleDict({'norm': LayerNorm(dims[1]),
+                                   'gated': GatedLinear(dims[1], 2 * dims[1]),
+                                   'back': Linear(2 * dims[1], dims[1])})
+            for layer in (block['gated'].gate, block['gated'].up, block['back']):
+                nn.init.xavier_normal_(layer.weight)
+            self.combined_blocks.append(block)
+            self.add_module(f'combined_block_{i}', block)
 
     def _configure_metadata_layers(self, metadata_type, layers_dims, num_cols) -> None:
         """``hybrid_pretrained_matrix_factorization.py:188-225``."""
@@ -284,7 +305,7 @@ class HybridPretrainedModel(MatrixFactorizationModel):
         # the layer LISTS are plain attributes in the reference too (the modules are registered
         # one by one through add_module)
         if name in ('item_metadata_layers', 'user_metadata_layers', 'combined_layers',
-                    'item_metadata', 'user_metadata'):
+                    'combined_blocks', 'item_metadata', 'user_metadata'):
             object.__setattr__(self, name, value)
         else:
             super().__setattr__(name, value)
@@ -405,10 +426,42 @@ class HybridPretrainedModel(MatrixFactorizationModel):
         if not (torch.is_grad_enabled() and params) and users.shape[0] > self._NO_GRAD_CHUNK:
             # scoring only (get_preds expands users x items pairs): bounded activation memory
             step = self._NO_GRAD_CHUNK
+            one = ((lambda u, i: self._head_forward(u, i)[0]) if not self.combined_blocks
+                   else self._block_forward)
             with torch.no_grad():
-                return torch.cat([self._head_forward(users[i:i + step], items[i:i + step])[0]
+                return torch.cat([one(users[i:i + step], items[i:i + step])
                                   for i in range(0, users.shape[0], step)]).squeeze()
+        if self.combined_blocks:
+            return self._block_forward(users, items).squeeze()
         return _HeadScore.apply(self, users, items, *params).squeeze()
+
+    def _block_forward(self, users, items):
+        """The head with residual blocks, layer by layer."""
+        status = self._status_flag()
+
+        def rows(table, ids):
+            return functional.embedding_rows(table, ids, status=status)
+
+        def metadata(kind, ids):
+            table = getattr(self, f'{kind}_metadata')
+            if table is None:
+                return []
+            x = rows(table, ids)
+            for layer in getattr(self, f'{kind}_metadata_layers') or ():
+                x = functional.linear(x, layer.weight, layer.bias, 'leaky_relu')
+            return [x]
+
+        x = torch.cat(metadata('user', users)
+                      + [rows(self.embeddings[0].weight, users),
+                         rows(self.embeddings[1].weight, items)]
+                      + metadata('item', items), dim=1)
+        for li, layer in enumerate(self.combined_layers[:-1]):
+            x = functional.linear(x, layer.weight, layer.bias, 'leaky_relu')
+            for block in self.combined_blocks if li == 0 else ():
+                x = block['back'](block['gated'](block['norm'](x)), residual=x)
+        last = self.combined_layers[-1]
+        bias = rows(self.biases[0].weight, users) + rows(self.biases[1].weight, items)
+        return functional.linear(x, last.weight, last.bias, residual=bias).reshape(-1)
 
     def calculate_loss(self, batch) -> torch.Tensor:
         """``base_pipeline.py:582-654``.  The positive and the K B negative pairs go through the
@@ -543,6 +596,7 @@ class HybridPretrainedModel(MatrixFactorizationModel):
         not allow the split (user metadata, a head of one layer): the caller then takes
         ``model(users, items)``."""
         if (self.user_metadata is not None or len(self.combined_layers) < 2 or n_items < 1
+                or self.combined_blocks
                 or (self.training and self.hparams.dropout_p > 0)):
             return None
         _lib.require_hip(self.embeddings[0].weight, 'HybridPretrainedModel')

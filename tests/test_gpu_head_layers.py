@@ -533,3 +533,84 @@ def test_another_stream_gives_the_same():
         second = torch.autograd.grad(y, params, torch.ones_like(y))
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+# ---- the hybrid model's head with residual blocks ------------------------------------------------
+def deep_hybrid(freeze, **kw):
+    from collie_amd.hybrid import HybridPretrainedModel
+    from collie_amd.model import MatrixFactorizationModel
+
+    class Shape:
+        num_users, num_items, num_negative_samples = 60, 40, 3
+
+    torch.manual_seed(2)
+    mf = MatrixFactorizationModel(train=Shape(), embedding_dim=10, lr_scheduler_func=None)
+    with torch.no_grad():
+        for t in (mf.user_embeddings, mf.item_embeddings, mf.user_biases, mf.item_biases):
+            t.weight.copy_(torch.randn(t.weight.shape))
+    model = HybridPretrainedModel(train=Shape(), item_metadata=torch.randn(40, 7),
+                                  user_metadata=torch.randn(60, 5), trained_model=mf,
+                                  item_metadata_layers_dims=[9], combined_layers_dims=[24, 12],
+                                  combined_blocks=2, freeze_embeddings=freeze,
+                                  lr_scheduler_func=None, **kw)
+    return model.to(DEV)
+
+
+def deep_reference(model, users, items):
+    """The same head in float64 torch on the CPU; returns (scores, {name: leaf})."""
+    p = {k: v.detach().cpu().double().requires_grad_(v.requires_grad)
+         for k, v in model.named_parameters()}
+
+    def lin(x, name):
+        return x @ p[name + '.weight'].T + p[name + '.bias']
+
+    leaky = torch.nn.functional.leaky_relu
+    x = torch.cat([model.user_metadata.cpu().double()[users], p['embeddings.0.weight'][users],
+                   p['embeddings.1.weight'][items],
+                   leaky(lin(model.item_metadata.cpu().double()[items], 'item_metadata_layer_0'))], 1)
+    x = leaky(lin(x, 'combined_layer_0'))
+    for i in range(2):
+        b = f'combined_block_{i}.'
+        h = torch.nn.functional.layer_norm(x, (24,), p[b + 'norm.weight'], p[b + 'norm.bias'])
+        h = torch.nn.functional.silu(lin(h, b + 'gated.gate')) * lin(h, b + 'gated.up')
+        x = lin(h, b + 'back') + x
+    x = leaky(lin(x, 'combined_layer_1'))
+    s = lin(x, 'combined_layer_2')[:, 0]
+    return s + p['biases.0.weight'][users, 0] + p['biases.1.weight'][items, 0], p
+
+
+@pytest.mark.parametrize('freeze', [True, False])
+def test_hybrid_head_with_blocks(freeze):
+    model = deep_hybrid(freeze, loss='bpr', optimizer='adam')
+    g = torch.Generator().manual_seed(9)
+    users, items = torch.randint(0, 60, (333,), generator=g), torch.randint(0, 40, (333,), generator=g)
+    c = rand((333,), torch.float32, 10)
+    scores = model(users.to(DEV), items.to(DEV))
+    (scores * c.to(DEV)).sum().backward()
+    want, p = deep_reference(model, users, items)
+    (want * c.double()).sum().backward()
+    # sixteen layers of at most 48 terms: their float32 roundings, in the 2-norm
+    room = 16 * 48 * hb.F
+    assert (scores.detach().cpu().double() - want).norm() <= room * want.norm()
+    for k, v in model.named_parameters():
+        if v.requires_grad:
+            assert (v.grad.cpu().double() - p[k].grad).norm() <= room * p[k].grad.norm(), k
+    # a training step as the trainers make it, and evaluation on the users x items grid
+    users, pos = users[:64].to(DEV), items[:64].to(DEV)
+    neg = torch.randint(0, 40, (64, 3), generator=g).to(DEV)
+    opt = model.configure_optimizers()
+    opt.zero_grad()
+    before = {k: v.detach().clone() for k, v in model.named_parameters()}
+    model.calculate_loss(((users, pos), neg)).backward()
+    opt.step()
+    for k, v in model.named_parameters():
+        assert torch.isfinite(v).all()
+        if v.requires_grad and k.startswith('combined_block'):
+            assert not torch.equal(v, before[k]), k
+    from collie_amd.metrics import get_preds
+    model.eval()
+    with torch.no_grad():
+        preds = get_preds(model, torch.arange(5), 40, DEV)
+        want, _ = deep_reference(model, torch.arange(5).repeat_interleave(40),
+                                 torch.arange(40).repeat(5))
+    assert (preds.reshape(-1).cpu().double() - want).norm() <= room * want.norm()

@@ -125,3 +125,41 @@ def test_c_entry_points_reject_bad_arguments():
     for i, call in enumerate(bad):
         assert call() == -1, i
         assert lib.collie_last_error()
+
+
+def _hybrid(**kw):
+    from collie_amd.hybrid import HybridPretrainedModel
+    from collie_amd.model import MatrixFactorizationModel
+
+    class Shape:
+        num_users, num_items, num_negative_samples = 30, 20, 3
+
+    torch.manual_seed(1)
+    mf = MatrixFactorizationModel(train=Shape(), embedding_dim=8, lr_scheduler_func=None)
+    return HybridPretrainedModel(train=Shape(), item_metadata=torch.ones(20, 6), trained_model=mf,
+                                 item_metadata_layers_dims=[12], combined_layers_dims=[16, 4],
+                                 lr_scheduler_func=None, **kw)
+
+
+def test_hybrid_head_with_blocks_is_built_saved_and_loaded(tmp_path):
+    from collie_amd.hybrid import HybridPretrainedModel
+    plain, deep = _hybrid(), _hybrid(combined_blocks=2)
+    more = set(deep.state_dict()) - set(plain.state_dict())
+    assert more == {f'combined_block_{i}.{n}.{p}' for i in range(2)
+                    for n in ('norm', 'gated.gate', 'gated.up', 'back') for p in ('weight', 'bias')}
+    assert deep.state_dict()['combined_block_1.gated.up.weight'].shape == (32, 16)
+    deep.save_model(tmp_path / 'deep')
+    loaded = HybridPretrainedModel(load_model_path=str(tmp_path / 'deep'))
+    for k, v in deep.state_dict().items():
+        assert torch.equal(v, loaded.state_dict()[k])
+    copy = _hybrid()
+    copy.load_from_hybrid_model(deep)
+    assert len(copy.combined_blocks) == 2
+    # a model saved before there were blocks
+    plain.hparams.pop('combined_blocks')
+    plain.save_model(tmp_path / 'plain')
+    assert HybridPretrainedModel(load_model_path=str(tmp_path / 'plain')).combined_blocks == []
+    with pytest.raises(ValueError, match='negative'):
+        _hybrid(combined_blocks=-1)
+    with pytest.raises(_lib.CollieHipError, match='no CPU fallback'):
+        deep(torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int64))
