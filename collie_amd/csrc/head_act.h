@@ -14,8 +14,8 @@ __device__ __forceinline__ float fast_exp(float x) {
   const float t = x * 1.44269504f;
   const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
   const float e = __builtin_amdgcn_exp2f(t);
-  // rest is not finite where t is not: e is 0 or infinite there already
-  return fabsf(t) < 200.0f ? fmaf(e, rest * 0.693147181f, e) : e;
+  // beyond, e is at an end of the range (infinite times a correction would be NaN)
+  return fabsf(t) < 126.0f ? fmaf(e, rest * 0.693147181f, e) : e;
 }
 __device__ __forceinline__ float fast_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z));

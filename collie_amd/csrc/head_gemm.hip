@@ -174,38 +174,48 @@ constexpr int64_t kSkinnyRows = 64;  // rows of the kernel that streams the weig
 constexpr int64_t kCus = 256;
 
 // A CU holds one workgroup of the 256 x 256 kernel or two of the 128 x 128 one (LDS).  The tiles that
-// fill whole rounds of the chip are computed as they are; those left over are cut along the depth, so
-// that they fill a round too: 344 tiles of 256 (a weight gradient of 11,008 x 2,048 over 16,384 rows)
-// took two rounds, 947 us.  The tile and the number of parts are the ones with the least time by
-// what a workgroup of either kernel was measured to do (products per second on large matrices), what
-// the parts' sums cost in memory traffic and what one more launch does.
+// fill whole rounds of the chip are computed as they are; those left over may be cut along the depth,
+// so that they fill a round too: 344 tiles of 256 (a weight gradient of 11,008 x 2,048 over 16,384
+// rows) took two rounds, 947 us, and take 745 cut.  Tile and parts are the ones with the least time by:
+// the products at the rate that all workgroups together reach on large matrices; the stores of a tile,
+// which all workgroups of a round make at about the same time, at a CU's share of a copy's bandwidth;
+// a start and an end of a few microseconds.  Against what was measured, large tile / small one
+// (us, bf16 with activation and kept values): 200,000 x 128 -> 256 110 / 95, 20,000 x 256 -> 256
+// 33 / 19, 8,192 x 1,024 -> 4,096 106 / 113.
 struct Plan {
   int tile;  // BM = BN
   int64_t tiles, full, splits, k_chunk;
 };
 
+// out_bytes: what is stored per accumulator
 template <typename T>
-Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair) {
+Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair, double out_bytes) {
   const int64_t depth = 128 / static_cast<int64_t>(sizeof(T));
   const int64_t stages = (k + depth - 1) / depth;
-  const double rate[2] = {sizeof(T) == 2 ? 0.9e15 : 1.6e14, sizeof(T) == 2 ? 1.04e15 : 1.9e14};
+  const double rate[2] = {sizeof(T) == 2 ? 0.95e15 : 1.78e14, sizeof(T) == 2 ? 1.1e15 : 2.24e14};
+  const double ends[2] = {1.5e-6, 3e-6};
+  const double cu_bandwidth = 4.7e12 / kCus;
   Plan best;
   double best_time = 0.0;
   for (int big = 0; big < 2; ++big) {
-    const int64_t t = big ? 256 : 128, slots = big ? kCus : 2 * kCus;
+    const int64_t t = big ? 256 : 128, per_cu = big ? 1 : 2, slots = kCus * per_cu;
     const int64_t tiles = ((m + t - 1) / t) * ((n * (pair ? 2 : 1) + t - 1) / t);
     const int64_t full = tiles / slots * slots, rest = tiles - full;
-    // of one tile: its products, and two stages' worth for the first load and the epilogue
-    const double one = 2.0 * t * t * static_cast<double>((stages + 2) * depth) * slots / rate[big];
+    const double stage = 2.0 * t * t * depth * slots / rate[big];
+    auto tile_time = [&](int64_t n_stages, double bytes) {
+      return n_stages * stage + per_cu * t * t * bytes / cu_bandwidth + ends[big];
+    };
     for (int64_t q = 0; q <= 4; ++q) {
       int64_t s = q == 0 || rest == 0 ? 1 : q * slots / rest;
-      if (s > stages / 4) s = stages / 4;
+      if (s > stages / 2) s = stages / 2;
       if (s < 1) s = 1;
       const int64_t part = (stages + s - 1) / s;
       s = (stages + part - 1) / part;
-      double time = one * (full / slots);
-      time += one * ((rest * s + slots - 1) / slots) * (part + 2) / (stages + 2);
-      if (s > 1) time += 5e-6 + 8.0 * s * rest * t * t / 4e12;
+      const int64_t rounds = (rest * s + slots - 1) / slots;
+      double time = tile_time(stages, out_bytes) * (full / slots);
+      time += rounds * tile_time(part, s > 1 ? 4.0 : out_bytes);
+      // the parts' sums are read again, by a launch of its own
+      if (s > 1) time += 4e-6 + (4.0 * s + out_bytes) * rest * t * t / 4e12;
       if ((big == 0 && q == 0) || time < best_time) {
         best_time = time;
         best = {static_cast<int>(t), tiles, s > 1 ? full : tiles, s, part * depth};
@@ -213,6 +223,12 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair) {
     }
   }
   return best;
+}
+
+// what the forward pass stores per accumulator when the backward pass is to follow
+template <typename T>
+double forward_bytes(bool pair) {
+  return pair ? (sizeof(T) + 8.0) / 2 : 2.0 * sizeof(T);
 }
 
 size_t partial_floats(const Plan& p) {
@@ -241,7 +257,8 @@ int launch_tile(const Gemm& g, const Plan& p, hipStream_t stream) {
 
 template <typename T, bool AKC, bool BKC, int EPI, bool CAT>
 int launch_tiles(Gemm& g, hipStream_t stream) {
-  const Plan p = plan_gemm<T>(g.m, g.n, g.k, EPI == kEpiGated);
+  constexpr bool PAIR = EPI == kEpiGated;
+  const Plan p = plan_gemm<T>(g.m, g.n, g.k, PAIR, EPI == kEpiStore ? sizeof(T) : forward_bytes<T>(PAIR));
   g.full = p.full;
   g.splits = static_cast<int>(p.splits);
   g.k_chunk = p.k_chunk;
@@ -296,7 +313,8 @@ FwdWs carve_fwd(void* base, const void* x, int64_t x_ld, int64_t m, int64_t n_in
     if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
     if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
     if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
-    ws.partial = c.take<float>(partial_floats(plan_gemm<T>(m, n_out, n_in, w2 != nullptr)));
+    ws.partial = c.take<float>(partial_floats(
+        plan_gemm<T>(m, n_out, n_in, w2 != nullptr, forward_bytes<T>(w2 != nullptr))));
   }
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;
@@ -324,8 +342,8 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
   if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
   if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
   ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m, n_out, kVec<T>)) * pair * n_out);
-  const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false));
-  const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false));
+  const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false, sizeof(T)));
+  const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false, sizeof(T)));
   ws.partial = c.take<float>(a > b ? a : b);
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;

@@ -19,7 +19,13 @@ def check(got, want, bound, dtype):
     assert got.dtype == dtype and got.shape == want.shape, (got.dtype, got.shape, want.shape)
     if want.numel() == 0:
         return
-    err = (got.double().cpu() - want).abs()
+    got = got.double().cpu()
+    # a value past the type's largest number is infinite: it must be where all of [want - bound,
+    # want + bound] is past it, and may be where some of it is
+    most = torch.finfo(dtype).max
+    inf = torch.isinf(got) & (want.abs() + bound > most) & (got.sign() * want + bound > most)
+    assert inf[want.abs() - bound > most].all()
+    err = torch.where(inf, torch.zeros_like(want), (got - want).abs())
     room = bound + U[dtype] * (want.abs() + bound) + TINY[dtype]
     worst = (err / room).max().item()
     assert torch.isfinite(err).all() and worst <= 1.0, f'error is {worst:.3g} of its bound'

@@ -300,6 +300,29 @@ def test_linear_activations(kind, dtype):
     run_linear(37, 48, 56, dtype, kind, True, False, seed=20)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('kind', ACTS)
+def test_activations_over_their_whole_range(kind, dtype):
+    """One input, weight one: z runs through the range, so every activation meets its ends."""
+    from collie_amd import functional as F
+    z = torch.cat([torch.linspace(-300, 300, 4801), torch.linspace(-3e4, 3e4, 101),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-5])]).to(dtype).reshape(-1, 1)
+    one, dy = torch.ones(1, 1, dtype=dtype), torch.ones_like(z)
+    x, w = leaf(z), leaf(one)
+    y = F.linear(x, w, activation=kind)
+    dx, dw = torch.autograd.grad(y, [x, w], dy.to(DEV))
+    ref = hb.linear(f64(z), f64(one), None, None, kind, f64(dy), dtype)
+    hb.check(y.detach(), *ref['y'], dtype)
+    hb.check(dx, *ref['dx'], dtype)
+    hb.check(dw, *ref['dw'], dtype)
+    y = F.gated_linear(x, w, w, activation=kind)
+    dx, dwg = torch.autograd.grad(y, [x, w], dy.to(DEV))
+    if dtype != torch.float16:      # (z^2 is past float16's range)
+        ref = hb.gated(f64(z), f64(one), f64(one), None, None, kind, f64(dy), dtype)
+        hb.check(y.detach(), *ref['y'], dtype)
+        hb.check(dx, *ref['dx'], dtype)
+
+
 def run_gated(m, n_in, n_out, dtype, kind, bias, seed=0):
     from collie_amd import functional as F
     std = n_in ** -0.5
