@@ -35,6 +35,7 @@ struct Gemm {
   void *c, *c2;          // output [m, n]; with kEpiStore rows >= row_split are c2's, and of either
   int64_t row_split;     // only the first row_valid are wanted
   int64_t row_valid;
+  bool stream;           // the results are stored past the caches
 };
 
 // biases of the columns col .. col + W
@@ -58,7 +59,7 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
   if constexpr (EPI == kEpiStore) {
     T* c = static_cast<T*>(row < g.row_split ? g.c : g.c2);
     const int64_t r = row < g.row_split ? row : row - g.row_split;
-    if (c && r < g.row_valid) store_pack<T, W>(c + r * g.n + col, left, v);
+    if (c && r < g.row_valid) store_pack<T, W>(c + r * g.n + col, left, v, g.stream);
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
@@ -68,12 +69,12 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
     float t[W];
     if (g.keep) {
       if constexpr (EPI == kEpiGated) {
-        store_pack<float, W>(static_cast<float*>(g.keep) + at, left, v);
-        store_pack<float, W>(static_cast<float*>(g.keep2) + at, left, u);
+        store_pack<float, W>(static_cast<float*>(g.keep) + at, left, v, g.stream);
+        store_pack<float, W>(static_cast<float*>(g.keep2) + at, left, u, g.stream);
       } else {
 #pragma unroll
         for (int j = 0; j < W; ++j) t[j] = kept<T>(v[j]);
-        store_pack<T, W>(static_cast<T*>(g.keep) + at, left, t);
+        store_pack<T, W>(static_cast<T*>(g.keep) + at, left, t, g.stream);
       }
     }
     act_values(g.act, v);
@@ -85,7 +86,7 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] += t[j];
     }
-    store_pack<T, W>(static_cast<T*>(g.c) + at, left, v);
+    store_pack<T, W>(static_cast<T*>(g.c) + at, left, v, g.stream);
   }
 }
 

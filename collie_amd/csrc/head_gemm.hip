@@ -24,6 +24,7 @@ struct ActBwd {
   int64_t m, n, dy_ld, dz_ld;
   int64_t rows_per_part;
   int act;
+  bool stream;             // dz is stored past the caches
 };
 constexpr int kActLanes = 32;
 constexpr int kActRows = kBlock / kActLanes;
@@ -66,8 +67,8 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
         T* dz = static_cast<T*>(p.dz) + row * p.dz_ld + col;
         const int64_t half = p.dz_ld / (PAIR ? 2 : 1);
         const int room = half - col < V ? static_cast<int>(half - col) : V;
-        store_pack<T, V>(dz, room, dy);
-        if (PAIR) store_pack<T, V>(dz + half, room, u);
+        store_pack<T, V>(dz, room, dy, p.stream);
+        if (PAIR) store_pack<T, V>(dz + half, room, u, p.stream);
       }
     }
   }
@@ -127,19 +128,30 @@ int sum_partials(const float* partial, int64_t count, int64_t width, int64_t spl
 // ---- laying an operand out for the tiles -----------------------------------------------------------
 // The tiles load whole aligned 16-byte packs.  Rows of another width or alignment are copied once
 // into rows of whole packs, zeros behind them: one more pass over that operand, for odd widths only.
+// All operands of a call go in one launch.
+struct PackJobs {
+  static constexpr int kMax = 4;
+  int n;
+  const void* src[kMax];
+  void* dst[kMax];
+  int64_t ld[kMax], cols[kMax], packs[kMax], total[kMax];  // packs per row, and in all
+};
+
 template <typename T>
-__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const T* __restrict__ src, int64_t ld,
-                                                           int64_t rows, int64_t cols, int64_t packs,
-                                                           T* __restrict__ dst) {
+__global__ __launch_bounds__(kBlock) void pack_rows_kernel(const PackJobs jobs) {
   constexpr int V = kVec<T>;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kBlock;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < rows * packs;
-       i += stride) {
-    const int64_t row = i / packs, c = (i - row * packs) * V;
-    const int64_t left = cols - c;
-    float v[V];
-    load_pack<T, V>(src + row * ld + c, left < V ? static_cast<int>(left) : V, v);
-    store_pack<T, V>(dst + i * V, V, v);
+  for (int k = 0; k < jobs.n; ++k) {
+    const T* src = static_cast<const T*>(jobs.src[k]);
+    T* dst = static_cast<T*>(jobs.dst[k]);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < jobs.total[k];
+         i += stride) {
+      const int64_t row = i / jobs.packs[k], c = (i - row * jobs.packs[k]) * V;
+      const int64_t left = jobs.cols[k] - c;
+      float v[V];
+      load_pack<T, V>(src + row * jobs.ld[k] + c, left < V ? static_cast<int>(left) : V, v);
+      store_pack<T, V>(dst + i * V, V, v);
+    }
   }
 }
 
@@ -155,17 +167,31 @@ int64_t padded(int64_t n) {
   return (n + kVec<T> - 1) / kVec<T> * kVec<T>;
 }
 
-// `p` laid out in rows of whole packs: itself, or its copy at `room`
+// `p` in rows of whole packs: itself, or its copy at `room`, which launch_packs() makes
 template <typename T>
-int lay_out(const void*& p, int64_t& ld, int64_t rows, int64_t cols, void* room, hipStream_t stream) {
-  if (whole_packs<T>(p, ld, cols)) return 0;
-  const int64_t packs = padded<T>(cols) / kVec<T>;
-  int64_t grid = (rows * packs + kBlock - 1) / kBlock;
-  if (grid > 8192) grid = 8192;
-  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(kBlock), 0, stream,
-                     static_cast<const T*>(p), ld, rows, cols, packs, static_cast<T*>(room));
+void lay_out(PackJobs& jobs, const void*& p, int64_t& ld, int64_t rows, int64_t cols, void* room) {
+  if (whole_packs<T>(p, ld, cols)) return;
+  const int k = jobs.n++;
+  jobs.src[k] = p;
+  jobs.dst[k] = room;
+  jobs.ld[k] = ld;
+  jobs.cols[k] = cols;
+  jobs.packs[k] = padded<T>(cols) / kVec<T>;
+  jobs.total[k] = rows * jobs.packs[k];
   p = room;
   ld = padded<T>(cols);
+}
+
+template <typename T>
+int launch_packs(const PackJobs& jobs, hipStream_t stream) {
+  if (jobs.n == 0) return 0;
+  int64_t grid = 1;
+  for (int k = 0; k < jobs.n; ++k) {
+    const int64_t blocks = (jobs.total[k] + kBlock - 1) / kBlock;
+    grid = grid > blocks ? grid : blocks;
+  }
+  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3(static_cast<unsigned>(grid < 8192 ? grid : 8192)),
+                     dim3(kBlock), 0, stream, jobs);
   return check_launch("pack_rows_kernel");
 }
 
@@ -207,7 +233,7 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair, double out_bytes) {
     };
     for (int64_t q = 0; q <= 4; ++q) {
       int64_t s = q == 0 || rest == 0 ? 1 : q * slots / rest;
-      if (s > stages / 2) s = stages / 2;
+      if (s > stages / 4) s = stages / 4;
       if (s < 1) s = 1;
       const int64_t part = (stages + s - 1) / s;
       s = (stages + part - 1) / part;
@@ -259,6 +285,7 @@ template <typename T, bool AKC, bool BKC, int EPI, bool CAT>
 int launch_tiles(Gemm& g, hipStream_t stream) {
   constexpr bool PAIR = EPI == kEpiGated;
   const Plan p = plan_gemm<T>(g.m, g.n, g.k, PAIR, EPI == kEpiStore ? sizeof(T) : forward_bytes<T>(PAIR));
+  g.stream = g.m * g.n * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
   g.full = p.full;
   g.splits = static_cast<int>(p.splits);
   g.k_chunk = p.k_chunk;
@@ -381,9 +408,12 @@ int layer_forward(const void* x, int64_t x_ld, const void* w, const void* w2, co
   if (m > kSkinnyRows) {
     const FwdWs ws = carve_fwd<T>(workspace, x, x_ld, m, n_in, w, w2, n_out);
     g.partial = ws.partial;
-    if (lay_out<T>(x, x_ld, m, n_in, ws.x, stream)) return -2;
-    if (lay_out<T>(w, ld, n_out, n_in, ws.w, stream)) return -2;
-    if (w2 && lay_out<T>(w2, ld2, n_out, n_in, ws.w2, stream)) return -2;
+    PackJobs jobs;
+    jobs.n = 0;
+    lay_out<T>(jobs, x, x_ld, m, n_in, ws.x);
+    lay_out<T>(jobs, w, ld, n_out, n_in, ws.w);
+    if (w2) lay_out<T>(jobs, w2, ld2, n_out, n_in, ws.w2);
+    if (launch_packs<T>(jobs, stream)) return -2;
   }
   g.a = {x, x_ld, 1};
   g.b = {w, ld, 1};
@@ -419,6 +449,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     if (z) {
       dz = p.dz = ws.dz;
       dz_ld = p.dz_ld = wide * half;
+      p.stream = m * dz_ld * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
     }
     p.partial = sums ? ws.act_partial : nullptr;
     const int64_t parts = act_parts(m, n_out, kVec<T>);
@@ -436,12 +467,18 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     }
   }
   if (!dx && !dw && !dw2) return 0;
-  if (!z && lay_out<T>(dz, dz_ld, m, n_out, ws.dz, stream)) return -2;
+  PackJobs jobs;
+  jobs.n = 0;
+  int64_t ld = n_in, ld2 = n_in;
+  if (!z) lay_out<T>(jobs, dz, dz_ld, m, n_out, ws.dz);
+  if (dx) {
+    lay_out<T>(jobs, w, ld, n_out, n_in, ws.w);
+    if (pair) lay_out<T>(jobs, w2, ld2, n_out, n_in, ws.w2);
+  }
+  if (dw || dw2) lay_out<T>(jobs, x, x_ld, m, n_in, ws.x);
+  if (launch_packs<T>(jobs, stream)) return -2;
   Gemm g;
   if (dx) {
-    int64_t ld = n_in, ld2 = n_in;
-    if (lay_out<T>(w, ld, n_out, n_in, ws.w, stream)) return -2;
-    if (pair && lay_out<T>(w2, ld2, n_out, n_in, ws.w2, stream)) return -2;
     memset(&g, 0, sizeof(g));
     g.a = {dz, dz_ld, 1};
     g.b = {w, 1, ld};
@@ -459,7 +496,6 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     if (rc) return rc;
   }
   if (dw || dw2) {
-    if (lay_out<T>(x, x_ld, m, n_in, ws.x, stream)) return -2;
     memset(&g, 0, sizeof(g));
     g.a = {dz, 1, dz_ld};
     g.b = {x, 1, x_ld};

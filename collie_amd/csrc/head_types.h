@@ -100,16 +100,21 @@ constexpr int64_t kStreamBytes = int64_t{64} << 20;
 
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* __restrict__ p, int n, const float (&v)[V], bool stream) {
-  static_assert(V * sizeof(T) == 16, "one 16-byte store");
   typedef uint32_t words __attribute__((ext_vector_type(4)));
-  if (stream && n >= V && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    Pack<T, V> a;
+  constexpr int N = kVec<T>;
+  if constexpr (V % N == 0) {
+    if (stream && n >= V && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = static_cast<T>(v[j]);
-    __builtin_nontemporal_store(__builtin_bit_cast(words, a), reinterpret_cast<words*>(p));
-  } else {
-    store_pack<T, V>(p, n, v);
+      for (int i = 0; i < V; i += N) {
+        Pack<T, N> a;
+#pragma unroll
+        for (int j = 0; j < N; ++j) a.v[j] = static_cast<T>(v[i + j]);
+        __builtin_nontemporal_store(__builtin_bit_cast(words, a), reinterpret_cast<words*>(p + i));
+      }
+      return;
+    }
   }
+  store_pack<T, V>(p, n, v);
 }
 
 // calls f.template operator()<T>() with the element type of a COLLIE_F32 / BF16 / F16 tag
