@@ -29,7 +29,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
-__device__ uint4 g_zero_chunk;  // what a load past the depth reads
+static __device__ uint4 g_zero_chunk;  // what a load past the depth reads
 
 // 16 bytes per lane from `g` to LDS at `lds` (wave-uniform) + 16 * lane.  In asm, because after the
 // builtin every later LDS read waits for all outstanding loads; the waits here are explicit.
@@ -48,7 +48,7 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-constexpr int kValu = 0x002, kMfma = 0x008, kDsRead = 0x100;  // groups of __builtin_amdgcn_sched_group_barrier
+constexpr int kMfma = 0x008, kDsRead = 0x100;  // groups of __builtin_amdgcn_sched_group_barrier
 
 // A fragment: 16 rows by 32 k; lane l holds row l % 16 and k = 8 (l / 16) + j.
 template <typename T>
@@ -135,6 +135,7 @@ struct Image {
 
   static __device__ __forceinline__ int swizzle(int row) {
     if (KC) return (row >> 1) & 7;
+    if (sizeof(T) == 2 && R == 64) return (((row >> 1) & 1) | ((row >> 2) & 2)) << 1;
     if (sizeof(T) == 2) return ((row & 3) | ((row >> 1) & 4)) << 1;
     return ((row >> 3) & 3) << 2;
   }
@@ -286,7 +287,7 @@ __device__ __forceinline__ void tile_at(int64_t id, int64_t tiles_m, int64_t til
 // a tile) after another, and the first stage of the next one is loaded under the last products and
 // the epilogue of the one before.
 template <typename T, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool CAT>
-__global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm g) {
+__global__ __launch_bounds__(kWave* WM* WN, BN == 64 ? 3 : 2) void gemm_tile_kernel(const Gemm g) {
   constexpr bool PAIR = EPI == kEpiGated;
   constexpr int THREADS = kWave * WM * WN;
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
@@ -347,7 +348,6 @@ __global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm 
     constexpr bool EXACT = decltype(exact)::value;
     const char* ib = ia + ImgA::kBytes;
     if constexpr (sizeof(T) == 4 && !EXACT) {
-      constexpr int RA32 = AKC ? 2 : 8, RB32 = BKC ? 2 : 8;
       Split b[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) b[j] = split(ImgB::read(ib, b_row(j), 0, lane));
@@ -356,19 +356,6 @@ __global__ __launch_bounds__(kWave* WM* WN, 2) void gemm_tile_kernel(const Gemm 
         const Split a = split(ImgA::read(ia, wm * (BM / WM) + i * 16, 0, lane));
 #pragma unroll
         for (int j = 0; j < NT; ++j) multiply(b[j], a, acc[i][j]);
-      }
-      // the split of the next row tile goes between the products of this one
-      __builtin_amdgcn_sched_group_barrier(kDsRead, RA32 + RB32 * NT, 0);
-      __builtin_amdgcn_sched_group_barrier(kValu, 46 * (NT + 1), 0);
-      __builtin_amdgcn_sched_group_barrier(kDsRead, RA32, 0);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int t = 0; t < 6 * NT; ++t) {
-          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kValu, 2, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(kDsRead, RA32, 0);
       }
     } else {
 #pragma unroll
@@ -607,21 +594,21 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
 // The parts of the depth of the cut tiles added in order, then the epilogue: 64 x 4 results of one
 // tile per workgroup; with SLICES > 1 the parts are shared out over the waves, whose sums are added
 // in order through LDS.
-template <typename T, int TILE, int EPI, int SLICES>
+template <typename T, int BM, int BN, int EPI, int SLICES>
 __global__ __launch_bounds__(kWave* SLICES) void gemm_finish_kernel(const Gemm g) {
   constexpr int NB = EPI == kEpiGated ? 2 : 1;
-  constexpr int TN = TILE / NB;
-  constexpr int kPacks = TILE * TN / 4;
+  constexpr int TN = BN / NB;
+  constexpr int kPacks = BM * TN / 4;
   const int lane = threadIdx.x & (kWave - 1), slice = threadIdx.x / kWave;
-  const int64_t tiles_m = (g.m + TILE - 1) / TILE, tiles_n = (g.n + TN - 1) / TN;
+  const int64_t tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + TN - 1) / TN;
   const int64_t rest = tiles_m * tiles_n - g.full;
   const int64_t tile = blockIdx.x / (kPacks / kWave);
   const int pack = blockIdx.x % (kPacks / kWave) * kWave + lane;
   const int lr = pack / (TN / 4), lc = pack % (TN / 4) * 4;
   int64_t tm, tn;
   tile_at(g.full + tile, tiles_m, tiles_n, tm, tn);
-  const int64_t row = tm * TILE + lr, col = tn * TN + lc;
-  const float* p = g.partial + (tile * NB * TILE + lr) * TN + lc;
+  const int64_t row = tm * BM + lr, col = tn * TN + lc;
+  const float* p = g.partial + (tile * NB * BM + lr) * TN + lc;
   f32x4 sum[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) sum[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -630,7 +617,7 @@ __global__ __launch_bounds__(kWave* SLICES) void gemm_finish_kernel(const Gemm g
     for (int s = slice; s < g.splits; s += SLICES)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        sum[b] += *reinterpret_cast<const f32x4*>(p + (s * rest * NB + b) * TILE * TN);
+        sum[b] += *reinterpret_cast<const f32x4*>(p + (s * rest * NB + b) * BM * TN);
   }
   if constexpr (SLICES > 1) {
     __shared__ f32x4 sh[SLICES][NB][kWave];
