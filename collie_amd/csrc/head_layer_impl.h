@@ -23,7 +23,8 @@ struct ActBwd {
   const void *dy;
   const void *z, *u;       // kept pre-activations: of the rows' type (NULL: identity), gated: float32
   void* dz;                // [m, dz_ld]; NULL: only the column sums are wanted
-  float* partial;          // [gridDim.y, pair * n] or NULL
+  float* partial;          // [gridDim.y, pair * n]: column sums, or NULL
+  void *db, *db2;          // gridDim.y = 1: the sums themselves (either may be NULL) instead
   int64_t m, n, dy_ld, dz_ld;
   int64_t rows_per_part;
   int act;
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
       }
     }
   }
-  if (p.partial == nullptr) return;
+  if (p.partial == nullptr && p.db == nullptr && p.db2 == nullptr) return;
   __shared__ float sh[kActRows][kActLanes * V];
 #pragma unroll
   for (int which = 0; which < (PAIR ? 2 : 1); ++which) {
@@ -89,7 +90,12 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
       float t = 0.0f;
 #pragma unroll
       for (int k = 0; k < kActRows; ++k) t += sh[k][c];
-      p.partial[(static_cast<int64_t>(blockIdx.y) * (PAIR ? 2 : 1) + which) * p.n + at] = t;
+      if (p.partial) {
+        p.partial[(static_cast<int64_t>(blockIdx.y) * (PAIR ? 2 : 1) + which) * p.n + at] = t;
+      } else {
+        T* db = static_cast<T*>(which ? p.db2 : p.db);
+        if (db) db[at] = static_cast<T>(t);
+      }
     }
   }
 }
@@ -329,6 +335,7 @@ int64_t act_parts(int64_t m, int64_t n, int64_t v) {
   const int64_t columns = (n + kActLanes * v - 1) / (kActLanes * v);
   int64_t parts = (2048 + columns - 1) / columns;
   if (parts < 64) parts = 64;
+  if (m <= 16 * kActRows) return 1;  // the sums at once: one launch less
   const int64_t most = (m + 4 * kActRows - 1) / (4 * kActRows);
   return parts < most ? parts : most;
 }
@@ -452,8 +459,13 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
       dz_ld = p.dz_ld = wide * half;
       p.stream = m * dz_ld * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
     }
-    p.partial = sums ? ws.act_partial : nullptr;
     const int64_t parts = act_parts(m, n_out, kVec<T>);
+    if (sums && parts > 1) {
+      p.partial = ws.act_partial;
+    } else {
+      p.db = db;
+      p.db2 = db2;
+    }
     p.rows_per_part = (m + parts - 1) / parts;
     const int64_t cols = kActLanes * kVec<T>;
     const dim3 grid(static_cast<unsigned>((n_out + cols - 1) / cols), static_cast<unsigned>(parts));
@@ -462,7 +474,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     else
       hipLaunchKernelGGL((act_bwd_kernel<T, false>), grid, dim3(kBlock), 0, stream, p);
     if (check_launch("act_bwd_kernel")) return -2;
-    if (sums) {
+    if (p.partial) {
       if (const int rc = sum_partials<T>(ws.act_partial, parts, wide * n_out, n_out, db, db2, stream))
         return rc;
     }

@@ -26,6 +26,7 @@ struct NormParams {
   float* mean;
   float* rstd;
   float* partial;    // backward: [workgroups, 2, dim] (NULL: not wanted)
+  void *dw, *db;     // backward with one workgroup: the sums themselves, of the parameters' type
   int64_t rows, x_ld, dy_ld;
   int dim;
   int w_f32;         // w and b are float32 (else: the rows' type)
@@ -181,31 +182,36 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const NormParams p) {
   }
   if (p.partial == nullptr) return;
   float* out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.dim;
-  if constexpr (G == 1) {
+  const bool last = gridDim.x == 1;
+  // the G rows that were worked on side by side, added in order
+  __shared__ float sh[G][TPR * NV * V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (left[i] > 0) {
-        store_pack<float, V>(out + col[i], left[i], dw[i]);
-        store_pack<float, V>(out + p.dim + col[i], left[i], db[i]);
-      }
-  } else {
-    // the G rows that were worked on side by side, added in order
-    __shared__ float sh[G][TPR * NV * V];
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
+  for (int which = 0; which < 2; ++which) {
+    void* final_out = which ? p.db : p.dw;
+    if (G == 1 && !last) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
+        if (left[i] > 0)
+          store_pack<float, V>(out + which * p.dim + col[i], left[i], which ? db[i] : dw[i]);
+      continue;
+    }
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          sh[threadIdx.x / TPR][(i * TPR + sub) * V + j] = which ? db[i][j] : dw[i][j];
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.dim; c += kBlock) {
-        float t = 0.0f;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int k = 0; k < G; ++k) t += sh[k][c];
+      for (int j = 0; j < V; ++j)
+        sh[threadIdx.x / TPR][(i * TPR + sub) * V + j] = which ? db[i][j] : dw[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.dim; c += kBlock) {
+      float t = 0.0f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) t += sh[k][c];
+      if (!last)
         out[which * p.dim + c] = t;
-      }
+      else if (final_out && p.w_f32)
+        static_cast<float*>(final_out)[c] = t;
+      else if (final_out)
+        static_cast<T*>(final_out)[c] = static_cast<T>(t);
     }
   }
 }
@@ -487,9 +493,12 @@ extern "C" int collie_layer_norm_backward(const void* dy, int64_t dy_ld, const v
     p.w_f32 = w_dtype == COLLIE_F32;
     p.stream = rows * dim * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
     const int count = rows ? norm_partials<T>(rows, dim) : 0;
+    p.dw = dweight;
+    p.db = dbias;
     const NormShape s = norm_shape<T>(dim);
     if (rows && s.tpr && (dx || sums)) {
       if (const int rc = launch_norm<T, true>(p, static_cast<unsigned>(count), stream)) return rc;
+      if (count == 1) return 0;  // the workgroup has written the sums
     } else if (rows) {
       if (dx) {
         hipLaunchKernelGGL(norm_dx_wide_kernel<T>, dim3(static_cast<unsigned>(rows < 8192 ? rows : 8192)),
