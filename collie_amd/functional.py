@@ -3,9 +3,14 @@ The layers of a deeper ranking head as differentiable functions of tensors on a 
 embedding rows with scaling, layer normalisation, the linear layer with bias, activation and
 residual, and the gated layer.  ``collie_amd.layers`` has them as modules.
 
-Inputs are float32, bfloat16 or float16 (all of one call alike); sums, statistics and activations
-are computed in float32 and every result is rounded once.  Gradients are summed in a fixed order:
-equal calls give equal bits.  There is no CPU fallback.
+Inputs are float32, bfloat16 or float16 (all of one call alike; under ``torch.autocast`` the caller
+casts); sums, statistics and activations are computed in float32 and every result is rounded once.
+Gradients are summed in a fixed order: equal calls give equal bits.  Layers other than the embedding
+rows can be differentiated once.  There is no CPU fallback.
+
+Everything is launched on the current stream of the inputs' device and can be captured into a graph.
+As with any torch operation, drop eager results that depend on the same leaves before a backward pass
+is captured: autograd would otherwise accumulate on the stream of the eager one.
 """
 import torch
 from torch.autograd.function import once_differentiable

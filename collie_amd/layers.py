@@ -19,9 +19,10 @@ from collie_amd import _lib, functional
 
 class _Table(torch.nn.Embedding):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
-        # what the kernels do not take (other devices and types, renormalised rows, gradients
-        # divided by counts) stays torch's
-        if (not self.weight.is_cuda or self.weight.dtype not in _lib.ELEMENT_TYPES
+        # what the kernels do not take (other devices and types, empty tables, renormalised rows,
+        # gradients divided by counts) stays torch's
+        if (not self.weight.is_cuda or self.weight.numel() == 0
+                or self.weight.dtype not in _lib.ELEMENT_TYPES
                 or not input.is_cuda or input.dtype not in (torch.int32, torch.int64)
                 or self.max_norm is not None or self.scale_grad_by_freq):
             return super().forward(input)

@@ -431,6 +431,40 @@ def test_layers_large_values():
         assert torch.isfinite(y[keep]).all()
 
 
+def test_float32_products_with_values_that_have_no_finite_parts():
+    """float32 products are made of bfloat16 parts; tiles with values that have none (infinities, NaN,
+    the top of the range) are computed again as they are.  Enough tiles that a workgroup works on
+    several: the others, before and after, stay what they are."""
+    from collie_amd import functional as F
+    a, b = rand((5200, 72), torch.float32, 70), rand((2600, 72), torch.float32, 71)
+    a[300, 5], a[1111, 70], a[5199, 0] = float('inf'), float('nan'), -float('inf')
+    a[2000] = 0.0
+    a[2000, 3] = 3.4e38                     # rounds up to no finite bfloat16
+    b[17] = 0.0
+    b[17, 3] = 0.5
+    y = F.linear(a.to(DEV), b.to(DEV)).cpu()
+    assert torch.isnan(y[1111]).all()
+    for row in (300, 5199):
+        k = 5 if row == 300 else 0
+        want = a[row, k] * b[:, k]          # +-inf by the sign of b, NaN where b is 0
+        assert torch.equal(torch.nan_to_num(y[row]), torch.nan_to_num(want))
+    assert y[2000, 17].item() == a[2000, 3].item() * 0.5
+    keep = torch.ones(5200, dtype=torch.bool)
+    keep[[300, 1111, 5199, 2000]] = False
+    val, bound = hb.product(a[keep].double(), b.double())
+    hb.check(y[keep], val, bound, torch.float32)
+    # the same through the gradients: dx has the bad rows, dW the bad columns, all of it
+    x, w = leaf(a), leaf(b)
+    dy = rand((5200, 2600), torch.float32, 72).to(DEV)
+    dx, dw = torch.autograd.grad(F.linear(x, w), [x, w], dy)
+    val, bound = hb.product(dy.cpu().double(), b.double().T)
+    hb.check(dx, val, bound, torch.float32)
+    good = [k for k in range(72) if k not in (0, 3, 5, 70)]
+    val, bound = hb.product(dy.cpu().double().T, a[:, good].double().T)
+    hb.check(dw[:, good], val, bound, torch.float32)
+    assert torch.isnan(dw[:, 70]).all() and torch.isinf(dw[:, [0, 5]]).all()
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_gradients_against_differences(dtype):
     """Directional derivatives of a loss through all operators, in float64 differences of the plain
