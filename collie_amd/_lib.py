@@ -5,6 +5,7 @@ There is no CPU fallback: every compute entry point of this package goes through
 raises ``CollieHipError`` if it cannot be loaded or a call fails.
 """
 import ctypes
+import importlib.util
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 
@@ -272,6 +273,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_autograd = None
 
 
 def lib_path():
@@ -295,6 +297,21 @@ def load():
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+def load_autograd():
+    """The extension module of the ranking-head operators (built next to the shared library)."""
+    global _autograd
+    if _autograd is None:
+        path = os.path.join(os.path.dirname(_LIB_PATH), '_head_autograd.so')
+        if not os.path.exists(path):
+            raise CollieHipError(f'{path} not found. Build it with ``make -C collie_amd/csrc``.')
+        load()
+        spec = importlib.util.spec_from_file_location('_head_autograd', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _autograd = module
+    return _autograd
 
 
 def check(rc, what):

@@ -3,7 +3,6 @@ Thin tensor-level wrappers over the C ABI: they only marshal torch tensors (devi
 current HIP stream) into ``libcollie_hip.so`` calls.  No arithmetic happens in this file.
 """
 import ctypes
-import functools
 from ctypes import byref, c_void_p
 
 import torch
@@ -931,154 +930,10 @@ def eval_merge_topk(cand_scores, cand_ids, k):
 
 
 # ---- layers of a deeper ranking head ---------------------------------------------------------------
-# These calls are short (a training step of a small batch makes many): pointers go to the entry
-# points as plain integers, and the backward forms rely on the checks of the forward ones.
-_cuda_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _call(t, name, *args):
-    """Entry point ``name`` on ``t``'s device and that device's current stream."""
-    index = t.get_device()
-    fn = getattr(load(), name)
-    if index == _cuda_device():
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        check(rc, name)
-
-
-def _at(t):
-    return None if t is None else t.data_ptr()
-
-
-def element_type(t, what):
-    tag = _lib.ELEMENT_TYPES.get(t.dtype)
-    if tag is None:
-        raise _lib.CollieHipError(f'{what} must be float32, bfloat16 or float16, not {t.dtype}')
-    return tag
-
-
-def rows_view(t, width):
-    """``t`` as [rows, width] with contiguous rows that do not overlap (a copy only if it must be),
-    and the distance of its rows in elements."""
-    if t.is_contiguous():
-        return (t if t.dim() == 2 else t.reshape(-1, width)), width
-    if t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
-        return t.contiguous().reshape(-1, width), width
-    return t, (t.stride(0) if t.shape[0] > 1 else width)
-
-
-@functools.lru_cache(maxsize=4096)
-def _bytes(name, *args):
-    """Workspace size ``name(*args)``.  Of addresses only the alignment counts: callers pass their
-    last four bits."""
-    return getattr(load(), name)(*args)
-
-
-def _workspace(like, name, *args):
-    """Scratch of one call (its caller holds it until the launches are in the stream)."""
-    return torch.empty(_bytes(name, *args), dtype=torch.uint8, device=like.device)
-
-
-def embedding_rows(table, ids, scale=1.0, status=None):
-    """``scale * table[ids]`` (``collie_embedding_rows``): [*ids.shape, dim]."""
-    require_hip(table, 'table')
-    require_hip(ids, 'ids')
-    tag = element_type(table, 'table')
-    if table.dim() != 2:
-        raise ValueError(f'table must be [rows, dim], not {tuple(table.shape)}')
-    if ids.device != table.device:
-        raise _lib.CollieHipError(f'ids are on {ids.device}, the table is on {table.device}')
-    table, ids = table.contiguous(), ids.contiguous()
-    rows, dim = table.shape
-    out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=table.device)
-    _call(table, 'collie_embedding_rows', table.data_ptr(), tag, rows, dim, ids.data_ptr(),
-          idx_dtype(ids), ids.numel(), scale, out.data_ptr(), _at(status))
-    return out
-
-
 def embedding_rows_grad(ids, dy, num_rows, scale=1.0, padding_idx=None, status=None):
-    """Gradient of ``embedding_rows`` with respect to the table, [num_rows, dim] in ``dy``'s type,
-    summed in the order of ``ids`` (``collie_embedding_rows_grad``)."""
-    require_hip(dy, 'dy')
-    require_hip(ids, 'ids')
-    tag = element_type(dy, 'dy')
-    dim = dy.shape[-1]
-    if dy.shape[:-1] != ids.shape:
-        raise ValueError(f'dy {tuple(dy.shape)} does not belong to ids {tuple(ids.shape)}')
-    if ids.device != dy.device:
-        raise _lib.CollieHipError(f'ids are on {ids.device}, dy is on {dy.device}')
-    n = ids.numel()
-    ids = ids.contiguous()
-    dy, ld = rows_view(dy, dim)
-    grad = torch.empty((num_rows, dim), dtype=dy.dtype, device=dy.device)
-    ws = _workspace(dy, 'collie_embedding_rows_grad_workspace_bytes', n, dim)
-    _call(dy, 'collie_embedding_rows_grad', ids.data_ptr(), idx_dtype(ids), n, dy.data_ptr(), ld, tag,
-          num_rows, dim, scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(),
-          ws.data_ptr(), ws.numel(), _at(status))
-    return grad
-
-
-def _param(t, like, shape, what, other=None):
-    """A parameter of a layer: on ``like``'s device, of its type (or ``other``), contiguous."""
-    if t is None:
-        return None
-    if t.shape != shape:
-        raise ValueError(f'{what} must have shape {tuple(shape)}, not {tuple(t.shape)}')
-    if t.device != like.device:
-        raise _lib.CollieHipError(f'{what} is on {t.device}, x is on {like.device}')
-    if t.dtype != like.dtype and t.dtype != other:
-        raise _lib.CollieHipError(f'{what} is {t.dtype}, x is {like.dtype}')
-    return t.contiguous()
-
-
-def layer_norm_forward(x, weight, bias, eps, keep):
-    """(y, mean, rstd) of ``collie_layer_norm_forward``; mean and rstd (per row, float32) only with
-    ``keep``."""
-    require_hip(x, 'x')
-    tag = element_type(x, 'x')
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f'x must have a last dimension to normalise, not {tuple(x.shape)}')
-    dim = x.shape[-1]
-    weight = _param(weight, x, (dim,), 'weight', torch.float32)
-    bias = _param(bias, x, (dim,), 'bias', torch.float32)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise _lib.CollieHipError(f'weight is {weight.dtype}, bias is {bias.dtype}')
-    rows, ld = rows_view(x, dim)
-    m = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, m), dtype=torch.float32, device=x.device) if keep else None
-    _call(x, 'collie_layer_norm_forward', rows.data_ptr(), ld, tag, m, dim, _at(weight), _at(bias),
-          _norm_param_tag(weight, bias, tag), eps, y.data_ptr(), _at(stats),
-          stats.data_ptr() + 4 * m if keep else None)
-    return y, stats
-
-
-def _norm_param_tag(weight, bias, tag):
-    given = weight if weight is not None else bias
-    return tag if given is None else _lib.ELEMENT_TYPES[given.dtype]
-
-
-def layer_norm_backward(dy, x, weight, bias, stats, want):
-    """(dx, dweight, dbias) of ``collie_layer_norm_backward`` from a forward call's arguments and
-    statistics, each None unless ``want`` says so."""
-    dim = x.shape[-1]
-    rows, ld = rows_view(x, dim)
-    dy, dy_ld = rows_view(dy, dim)
-    m = rows.shape[0]
-    tag = _lib.ELEMENT_TYPES[x.dtype]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
-    dw, db = (torch.empty((dim,), dtype=p.dtype, device=x.device) if w and p is not None else None
-              for w, p in zip(want[1:], (weight, bias)))
-    ws = _workspace(x, 'collie_layer_norm_backward_workspace_bytes', m, dim)
-    _call(x, 'collie_layer_norm_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, dim,
-          _at(weight.contiguous() if weight is not None else None),
-          _norm_param_tag(weight, bias, tag), stats.data_ptr(), stats.data_ptr() + 4 * m, _at(dx),
-          _at(dw), _at(db), ws.data_ptr(), ws.numel())
-    return dx, dw, db
+    """Gradient of ``functional.embedding_rows`` with respect to the table, [num_rows, dim] in ``dy``'s
+    type, summed in the order of ``ids`` (``collie_embedding_rows_grad``)."""
+    return _lib.load_autograd().embedding_rows_grad(ids, dy, num_rows, scale, padding_idx, status)
 
 
 def activation_code(name):
@@ -1086,113 +941,3 @@ def activation_code(name):
     if code is None:
         raise ValueError(f'{name!r} is not an activation: {", ".join(_lib.ACTIVATIONS)}')
     return code
-
-
-def _layer_args(x, weight, biases, second=None):
-    """Checked (element type, rows of x, their distance, weights, biases) of a layer."""
-    require_hip(x, 'x')
-    tag = element_type(x, 'x')
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f'x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit: expected '
-                         'x [..., n_in] and weight [n_out, n_in]')
-    n_out, n_in = weight.shape
-    if n_out < 1 or n_in < 1:
-        raise ValueError(f'weight {tuple(weight.shape)} is empty')
-    weights = [_param(weight, x, weight.shape, 'weight')]
-    if second is not None:
-        weights.append(_param(second, x, weight.shape, 'weight'))
-    biases = [_param(b, x, (n_out,), 'bias') for b in biases]
-    rows, ld = rows_view(x, n_in)
-    return tag, rows, ld, weights, biases
-
-
-def _param_rows(t, like, shape, what):
-    if t.shape != shape:
-        raise ValueError(f'{what} must have shape {tuple(shape)}, not {tuple(t.shape)}')
-    if t.device != like.device or t.dtype != like.dtype:
-        raise _lib.CollieHipError(f'{what} is {t.dtype} on {t.device}, x is {like.dtype} on '
-                                  f'{like.device}')
-    return t
-
-
-def linear_forward(x, weight, bias, activation, residual, keep):
-    """(y, kept pre-activations or None) of ``collie_linear_forward``."""
-    act = activation_code(activation)
-    tag, rows, ld, (weight,), (bias,) = _layer_args(x, weight, (bias,))
-    n_out, n_in = weight.shape
-    m = rows.shape[0]
-    shape = (*x.shape[:-1], n_out)
-    res, res_ld = None, 0
-    if residual is not None:
-        res, res_ld = rows_view(_param_rows(residual, x, shape, 'residual'), n_out)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    kept = torch.empty((m, n_out), dtype=x.dtype, device=x.device) if keep and act else None
-    ws = _workspace(x, 'collie_layer_forward_workspace_bytes', rows.data_ptr() & 15, ld, tag, m, n_in,
-                    weight.data_ptr() & 15, None, n_out)
-    _call(x, 'collie_linear_forward', rows.data_ptr(), ld, tag, m, n_in, weight.data_ptr(), _at(bias),
-          n_out, act, _at(res), res_ld, _at(kept), y.data_ptr(), ws.data_ptr(), ws.numel())
-    return y, kept
-
-
-def linear_backward(dy, x, weight, activation, kept, want):
-    """(dx, dweight, dbias) of ``collie_linear_backward`` from a forward call's arguments and what it
-    kept, each None unless ``want`` says so."""
-    n_out, n_in = weight.shape
-    rows, ld = rows_view(x, n_in)
-    m = rows.shape[0]
-    make = torch.empty if m else torch.zeros
-    dx, dw, db = (make(s, dtype=x.dtype, device=x.device) if w else None for w, s in
-                  zip(want, (x.shape, (n_out, n_in), (n_out,))))
-    if m == 0:
-        return dx, dw, db
-    weight = weight.contiguous()
-    dy, dy_ld = rows_view(dy, n_out)
-    tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
-    ws = _workspace(x, 'collie_layer_backward_workspace_bytes', dy.data_ptr() & 15, dy_ld,
-                    rows.data_ptr() & 15, ld, tag, m, n_in, weight.data_ptr() & 15, None, n_out, act)
-    _call(x, 'collie_linear_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
-          weight.data_ptr(), n_out, act, _at(kept), _at(dx), _at(dw), _at(db),
-          ws.data_ptr(), ws.numel())
-    return dx, dw, db
-
-
-def gated_forward(x, gate_weight, up_weight, gate_bias, up_bias, activation, keep):
-    """(y, kept gate, kept up) of ``collie_gated_forward``; the kept ones None without ``keep``."""
-    act = activation_code(activation)
-    if (gate_bias is None) != (up_bias is None):
-        raise ValueError('gate_bias and up_bias: both or none')
-    tag, rows, ld, (wg, wu), (bg, bu) = _layer_args(x, gate_weight, (gate_bias, up_bias), up_weight)
-    n_out, n_in = wg.shape
-    m = rows.shape[0]
-    y = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=x.device)
-    g = u = None
-    if keep:
-        g, u = torch.empty((2, m, n_out), dtype=torch.float32, device=x.device)
-    ws = _workspace(x, 'collie_layer_forward_workspace_bytes', rows.data_ptr() & 15, ld, tag, m, n_in,
-                    wg.data_ptr() & 15, 16 | wu.data_ptr() & 15, n_out)
-    _call(x, 'collie_gated_forward', rows.data_ptr(), ld, tag, m, n_in, wg.data_ptr(), wu.data_ptr(),
-          _at(bg), _at(bu), n_out, act, _at(g), _at(u), y.data_ptr(), ws.data_ptr(), ws.numel())
-    return y, g, u
-
-
-def gated_backward(dy, x, gate_weight, up_weight, activation, kept_gate, kept_up, want):
-    """(dx, dgate_weight, dup_weight, dgate_bias, dup_bias) of ``collie_gated_backward`` from a
-    forward call's arguments and what it kept, each None unless ``want`` says so."""
-    n_out, n_in = gate_weight.shape
-    rows, ld = rows_view(x, n_in)
-    m = rows.shape[0]
-    make = torch.empty if m else torch.zeros
-    shapes = (x.shape, (n_out, n_in), (n_out, n_in), (n_out,), (n_out,))
-    out = [make(s, dtype=x.dtype, device=x.device) if w else None for w, s in zip(want, shapes)]
-    if m == 0:
-        return out
-    wg, wu = gate_weight.contiguous(), up_weight.contiguous()
-    dy, dy_ld = rows_view(dy, n_out)
-    tag, act = _lib.ELEMENT_TYPES[x.dtype], _lib.ACTIVATIONS[activation]
-    ws = _workspace(x, 'collie_layer_backward_workspace_bytes', dy.data_ptr() & 15, dy_ld,
-                    rows.data_ptr() & 15, ld, tag, m, n_in, wg.data_ptr() & 15,
-                    16 | wu.data_ptr() & 15, n_out, act)
-    _call(x, 'collie_gated_backward', dy.data_ptr(), dy_ld, rows.data_ptr(), ld, tag, m, n_in,
-          wg.data_ptr(), wu.data_ptr(), n_out, act, kept_gate.data_ptr(), kept_up.data_ptr(),
-          *[_at(t) for t in out], ws.data_ptr(), ws.numel())
-    return out

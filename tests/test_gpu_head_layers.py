@@ -122,6 +122,40 @@ def test_embedding_rows_second_derivative_and_sparse_gradient():
     assert torch.equal(sp.to_dense().cpu(), ref)
 
 
+def test_layers_other_than_the_rows_refuse_a_second_derivative():
+    from collie_amd import functional as F
+    x, w, b = (leaf(rand(s, torch.float32, i)) for i, s in enumerate([(3, 4), (5, 4), (5,)]))
+    for y in (F.linear(x, w, b, 'silu'), F.gated_linear(x, w, w), F.layer_norm(x, w[0], w[1])):
+        (g,) = torch.autograd.grad(y.sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError, match='differentiated once'):
+            torch.autograd.grad(g.sum(), [x])
+    # only what is asked for is computed, and a residual's gradient may be differentiated again
+    r = leaf(rand((3, 5), torch.float32, 4))
+    y = F.linear(x.detach(), w.detach(), residual=r)
+    (g,) = torch.autograd.grad((y ** 2).sum(), [r], create_graph=True)
+    assert torch.equal(torch.autograd.grad(g.sum(), [r])[0], torch.full_like(r, 2.0))
+    y = F.linear(x, w, b, 'gelu', r)
+    every = torch.autograd.grad(y, [x, w, b, r], torch.ones_like(y), retain_graph=True)
+    for leaf_of, g in zip((x, w, b, r), every):
+        (one,) = torch.autograd.grad(y, [leaf_of], torch.ones_like(y), retain_graph=True)
+        assert torch.equal(one, g)
+
+
+def test_embedding_status_may_be_cleared_between_the_passes():
+    from collie_amd import functional as F
+    w = leaf(rand((6, 4), torch.float32, 6))
+    ids = torch.tensor([5, 6, -1, 2], device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    y = F.embedding_rows(w, ids, status=status)
+    assert status.item() == 1
+    status.zero_()
+    (g,) = torch.autograd.grad(y, [w], torch.ones_like(y))
+    assert status.item() == 1
+    ref = torch.zeros(6, 4)
+    ref[5], ref[2] = 1.0, 1.0
+    assert torch.equal(g.cpu(), ref)
+
+
 @pytest.mark.parametrize('cls', ['ScaledEmbedding', 'ZeroEmbedding'])
 @pytest.mark.parametrize('sparse', [False, True])
 def test_table_modules_give_what_torch_gives(cls, sparse):

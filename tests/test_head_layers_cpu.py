@@ -54,29 +54,47 @@ def test_refusals_before_any_launch():
         F.embedding_rows(w, torch.zeros(1, dtype=torch.int64), padding_idx=3)
     with pytest.raises(_lib.CollieHipError, match='status'):
         F.embedding_rows(w, torch.zeros(1, dtype=torch.int64), status=torch.zeros(1))
-    with pytest.raises(ValueError, match='shape'):
-        ops._param(torch.zeros(1, 3), x, (3,), 'bias')
-    with pytest.raises(_lib.CollieHipError, match='bias is'):
-        ops._param(torch.zeros(3, dtype=torch.float64), x, (3,), 'bias')
+    for call in (lambda: F.linear(x, w, torch.zeros(1, 3)), lambda: F.layer_norm(x, torch.zeros(3)),
+                 lambda: F.gated_linear(x, w, torch.zeros(4, 3))):
+        with pytest.raises(ValueError, match='must have shape'):
+            call()
+    with pytest.raises(ValueError, match='do not fit'):
+        F.linear(x, torch.zeros(3, 5))
+    with pytest.raises(ValueError, match='is empty'):
+        F.linear(x, torch.zeros(0, 4))
+    with pytest.raises(_lib.CollieHipError, match='bias is torch.float64, x is torch.float32'):
+        F.linear(x, w, torch.zeros(3, dtype=torch.float64))
+    with pytest.raises(_lib.CollieHipError, match='weight is torch.float32, bias is torch.bfloat16'):
+        F.layer_norm(x.bfloat16(), torch.ones(4), torch.zeros(4, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match='residual must have shape'):
-        ops._param_rows(torch.zeros(1, 3), x, (2, 3), 'residual')
+        F.linear(x, w, residual=torch.zeros(1, 3))
     with pytest.raises(_lib.CollieHipError, match='residual is'):
-        ops._param_rows(torch.zeros(2, 3, dtype=torch.bfloat16), x, (2, 3), 'residual')
+        F.linear(x, w, residual=torch.zeros(2, 3, dtype=torch.bfloat16))
     with pytest.raises(_lib.CollieHipError, match='float64'):
-        ops.element_type(torch.zeros(1, dtype=torch.float64), 'x')
+        F.layer_norm(x.double())
+    with pytest.raises(_lib.CollieHipError, match='index tensors'):
+        F.embedding_rows(w, torch.zeros(2, dtype=torch.int16))
+    for call in (lambda v: F.embedding_rows(v, torch.zeros(2, dtype=torch.int64)),
+                 lambda v: F.layer_norm(v), lambda v: F.linear(v, v), lambda v: F.linear(x[:, :1], v.t()),
+                 lambda v: ops.embedding_rows_grad(torch.zeros(1, dtype=torch.int64), v, 3)):
+        with pytest.raises(ValueError, match='too wide'):
+            call(torch.zeros(1, 1).expand(1, (1 << 32) + 8))
+    with pytest.raises(ValueError, match='does not belong'):
+        ops.embedding_rows_grad(torch.zeros(3, dtype=torch.int64), x, 5)
 
 
 def test_rows_view_copies_only_what_it_must():
+    rows_view = _lib.load_autograd().rows_view
     base = torch.arange(60.0).reshape(5, 12)
-    t, ld = ops.rows_view(base[:, 2:9], 7)
+    t, ld = rows_view(base[:, 2:9], 7)
     assert t.data_ptr() == base[:, 2:].data_ptr() and ld == 12
     for view in (base.t(), base[:1, :7].expand(5, 7), base[:, ::2],
                  base.reshape(5, 3, 4)[:, 1:, :], base.as_strided((4, 8), (3, 1))):
-        t, ld = ops.rows_view(view, view.shape[-1])
+        t, ld = rows_view(view, view.shape[-1])
         assert t.is_contiguous() and ld == t.shape[1]
         assert torch.equal(t.reshape(view.shape), view)
-    assert ops.rows_view(torch.zeros(7), 7)[0].shape == (1, 7)
-    assert ops.rows_view(torch.zeros(0, 3, 7), 7)[0].shape == (0, 7)
+    assert rows_view(torch.zeros(7), 7)[0].shape == (1, 7)
+    assert rows_view(torch.zeros(0, 3, 7), 7)[0].shape == (0, 7)
 
 
 def test_c_entry_points_reject_bad_arguments():
