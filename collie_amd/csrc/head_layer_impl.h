@@ -213,11 +213,13 @@ constexpr int64_t kCus = 256;
 // fill whole rounds of the chip are computed as they are; those left over may be cut along the depth,
 // so that they fill a round too: 344 tiles of 256 (a weight gradient of 11,008 x 2,048 over 16,384
 // rows) took two rounds, 947 us, and take 745 cut.  Tile and parts are the ones with the least time by:
-// the products at the rate that all workgroups together reach on large matrices; the stores of a tile,
-// which all workgroups of a round make at about the same time, at a CU's share of a copy's bandwidth;
-// a start and an end of a few microseconds.  Against what was measured, large tile / small one
-// (us, bf16 with activation and kept values): 200,000 x 128 -> 256 110 / 95, 20,000 x 256 -> 256
-// 33 / 19, 8,192 x 1,024 -> 4,096 106 / 113.
+// the products at the rate that all workgroups together reach on large matrices; the stores of a tile
+// at a CU's share of a copy's bandwidth (of the workgroups that share a CU one stores while the others
+// multiply, so that only its own stores count); a start and an end of a few microseconds.  Against what
+// was measured, 128 x 64 / 128 x 128 / 256 x 256 (us): float32 720,896 x 128 -> 256 528 / 463 / 517,
+// 200,000 x 256 -> 512 445 / 378 / 431, 65,536 x 1,024 -> 512 492 / 398 / 402, 16,384 x 2,048 -> 5,504
+// 2,535 / 2,052 / 1,825; bfloat16 20,000 x 256 -> 256 with kept values 17 / 21 / 34, 720,896 x 64 -> 128
+// 56 / 61 / 92, 8,192 x 1,024 -> 4,096 103 / 79 / 84, gated 16,384 x 2,048 -> 5,504 970 / 810 / 757.
 struct Plan {
   int bm, bn;
   int64_t slots;  // workgroups that the chip holds
@@ -233,9 +235,9 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair, double out_bytes) {
     int bm, bn, per_cu;
     double rate16, rate32, ends;
   };
-  static const Shape shapes[] = {{128, 64, 3, 0.55e15, 1.42e14, 1.2e-6},
-                                 {128, 128, 2, 0.95e15, 1.78e14, 1.5e-6},
-                                 {256, 256, 1, 1.1e15, 2.24e14, 3e-6}};
+  static const Shape shapes[] = {{128, 64, 3, 0.72e15, 1.48e14, 1.2e-6},
+                                 {128, 128, 2, 0.95e15, 1.95e14, 1.5e-6},
+                                 {256, 256, 1, 1.12e15, 2.24e14, 3e-6}};
   const double cu_bandwidth = 4.7e12 / kCus;
   Plan best;
   memset(&best, 0, sizeof(best));
@@ -247,7 +249,7 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair, double out_bytes) {
     const double area = static_cast<double>(c.bm) * c.bn;
     const double stage = 2.0 * area * depth * slots / (sizeof(T) == 2 ? c.rate16 : c.rate32);
     auto tile_time = [&](int64_t n_stages, double bytes) {
-      return n_stages * stage + c.per_cu * area * bytes / cu_bandwidth + c.ends;
+      return n_stages * stage + area * bytes / cu_bandwidth + c.ends;
     };
     for (int64_t q = 0; q <= 4; ++q) {
       int64_t s = q == 0 || rest == 0 ? 1 : q * slots / rest;
