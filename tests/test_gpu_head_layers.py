@@ -705,3 +705,77 @@ def test_hybrid_head_with_blocks(freeze):
         want, _ = deep_reference(model, torch.arange(5).repeat_interleave(40),
                                  torch.arange(40).repeat(5))
     assert (preds.reshape(-1).cpu().double() - want).norm() <= room * want.norm()
+
+
+def _pass(F, p, call=None):
+    """One block with its gradients."""
+    leaves = [t.detach().requires_grad_() for t in p]
+    table, norm_w, wg, wu, back, bias = leaves
+
+    def block(table):
+        h = F.embedding_rows(table, torch.arange(40, device=DEV) % table.shape[0], scale=0.5)
+        g = F.gated_linear(F.layer_norm(h, norm_w), wg, wu)
+        return F.linear(g, back, bias, 'gelu', residual=h)
+
+    y = call(block, table) if call else block(table)
+    return [y, *torch.autograd.grad((y * y).sum(), leaves)]
+
+
+def _block_parameters():
+    shapes = [(17, 24), (24,), (36, 24), (36, 24), (24, 36), (24,)]
+    return [rand(s, torch.float32, 70 + i).to(DEV) for i, s in enumerate(shapes)]
+
+
+def test_saved_tensors_may_be_packed_or_computed_again():
+    from torch.utils.checkpoint import checkpoint
+
+    from collie_amd import functional as F
+    p = _block_parameters()
+    ref = _pass(F, p)
+    again = _pass(F, p, lambda block, t: checkpoint(block, t, use_reentrant=False))
+    with torch.autograd.graph.save_on_cpu():
+        packed = _pass(F, p)
+    for other in (again, packed):
+        assert all(torch.equal(a, b) for a, b in zip(ref, other))
+
+
+def test_threads_on_streams_of_their_own_give_the_same():
+    from concurrent.futures import ThreadPoolExecutor
+
+    from collie_amd import functional as F
+    p = _block_parameters()
+    ref = _pass(F, p)
+    torch.cuda.synchronize()
+
+    def work(_):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            out = [_pass(F, p) for _ in range(5)]
+        stream.synchronize()
+        return out
+
+    with ThreadPoolExecutor(4) as pool:
+        for results in pool.map(work, range(4)):
+            for other in results:
+                assert all(torch.equal(a, b) for a, b in zip(ref, other))
+
+
+def test_a_captured_block_replays_with_eager_work_between():
+    from collie_amd import functional as F
+    p = _block_parameters()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            _pass(F, p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        captured = _pass(F, p)
+    for turn in range(3):
+        for t in p:
+            t.mul_(1.0 + 0.25 * turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = _pass(F, p)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager))
