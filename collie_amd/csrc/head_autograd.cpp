@@ -217,14 +217,15 @@ variable_list Lookup::backward(AutogradContext* ctx, variable_list grads) {
   const int64_t rows = rest[0], padding = rest[1];
   Tensor dw;
   if (rest[2]) {
-    // the uncoalesced COO gradient of nn.Embedding(sparse=True)
+    // the uncoalesced COO gradient of nn.Embedding(sparse=True), without entries that take no gradient: an
+    // index outside the table would be an address outside of it for whoever uses the tensor
     Tensor flat = ids.reshape({-1}).to(at::kLong), vals = grads[0].reshape({-1, grads[0].size(-1)});
+    Tensor live = flat.ge(0).logical_and(flat.lt(rows));
+    if (padding >= 0) live = live.logical_and(flat.ne(padding));
+    const Tensor which = live.nonzero().reshape({-1});
+    flat = flat.index_select(0, which);
+    vals = vals.index_select(0, which);
     if (scale != 1.0) vals = vals * scale;
-    if (padding >= 0) {
-      const Tensor live = flat != padding;
-      flat = flat.masked_select(live);
-      vals = vals.index({live});
-    }
     dw = at::sparse_coo_tensor(flat.unsqueeze(0), vals, {rows, vals.size(1)});
   } else if (at::GradMode::is_enabled()) {
     dw = LookupGrad::apply(grads[0], ids, status, rows, scale, padding);
