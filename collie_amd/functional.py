@@ -29,18 +29,24 @@ def embedding_rows(weight, ids, scale=1.0, padding_idx=None, sparse=False, statu
 
 # Rows from which on a table's dense gradient is summed by sorted ids.  Below, the handful of launches
 # costs more than torch's atomic adds even on skewed ids (11,264 x 128 into 138,493 rows: 63 us sorted,
-# 19 us uniform and 53 us skewed with atomics); above, skewed ids meet on a few rows and the adds queue
-# up (65,536 x 128: 71 us sorted, 43 and 251 us with atomics; 720,896 x 128: 164 us against 2.6 ms).
+# 23 us uniform and 57 us skewed with atomics, 9 us of each for the check of the ids); above, skewed ids
+# meet on a few rows and the adds queue up (65,536 x 128: 70 us sorted, 51 and 264 us with atomics;
+# 720,896 x 128: 164 us against 2.6 ms).
 SORTED_GRAD_ROWS = 65536
 
 
 def table_grad(table, ids, vals, status=None):
     """Dense gradient of ``table`` (float32) from one row of ``vals`` per id, as ``nn.Embedding``
-    gives it; many rows are summed by sorted ids, in the order of the batch."""
+    gives it; many rows are summed by sorted ids, in the order of the batch.  Ids outside the table
+    take no gradient (the lookup has set bit 0 of ``status`` for them)."""
+    rows = table.shape[0]
     vals = vals.reshape(ids.shape[0], table.shape[1])
     if ids.shape[0] < SORTED_GRAD_ROWS:
-        return torch.zeros_like(table).index_add_(0, ids.long(), vals)
-    return ops.embedding_rows_grad(ids, vals, table.shape[0], status=status)
+        # index_add_ does not look at the ids on every build of torch: those outside the table (-1 and
+        # `rows` after the clamp, `rows` after the remainder) go to a row behind it
+        inside = ids.long().clamp(-1, rows).remainder_(rows + 1)
+        return table.new_zeros(rows + 1, table.shape[1]).index_add_(0, inside, vals)[:rows]
+    return ops.embedding_rows_grad(ids, vals, rows, status=status)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
