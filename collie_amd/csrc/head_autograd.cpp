@@ -5,10 +5,12 @@
 // own thread, took several times as long as the launches.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -44,6 +46,33 @@ void require_hip(const Tensor& t, const char* what) {
   REFUSE(!t.is_cuda(), what, ": tensor is on ", t.device(),
          "; collie_amd computes on a HIP device only (no CPU fallback). Move the model and data with "
          "``.to(\"cuda\")``.");
+}
+
+// The kernels see memory.  A tensor that stands for something else (a batch of vmap, a subclass such as a
+// fake tensor), one with a tangent of forward-mode differentiation, and any tensor while a graph is
+// being recorded from torch's own calls, would lose that silently.
+bool plain(const Tensor& t) {
+  using c10::DispatchKey;
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  static const c10::DispatchKeySet wrapped({DispatchKey::Python, DispatchKey::FuncTorchBatched,
+                                            DispatchKey::FuncTorchGradWrapper,
+                                            DispatchKey::Functionalize});
+  if (t.key_set().has_any(wrapped) || !t.has_storage() || t._fw_grad(0).defined()) return false;
+  return !torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) &&
+         !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) &&
+         !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL);
+}
+
+void require_plain(const MaybeTensor& t) {
+  REFUSE(t && t->defined() && !plain(*t),
+         "collie_amd computes on memory: tensors under vmap, torch.func or torch.jit.trace, fake tensors and "
+         "tensors with a forward-mode tangent are not supported");
+}
+template <typename... Rest>
+void require_plain(const MaybeTensor& t, const Rest&... rest) {
+  require_plain(t);
+  require_plain(rest...);
 }
 
 std::string dtype(const Tensor& t) {
@@ -174,6 +203,32 @@ Tensor lookup_grad(const Tensor& ids, const Tensor& dy, int64_t num_rows, double
   return grad;
 }
 
+// The same for tensors that are not plain (a gradient under vmap or with a forward-mode tangent), in
+// torch's operations: ids outside the table go to a row of zeros behind it.
+Tensor inside(const Tensor& ids, int64_t num_rows) {
+  return ids.reshape({-1}).to(at::kLong).clamp(-1, num_rows).remainder(num_rows + 1);
+}
+
+Tensor plain_lookup(const Tensor& table, const Tensor& ids, double scale) {
+  auto shape = ids.sizes().vec();
+  shape.push_back(table.size(1));
+  const Tensor rows = at::cat({table, at::zeros({1, table.size(1)}, table.options())});
+  return (rows.index_select(0, inside(ids, table.size(0))).to(at::kFloat) * scale)
+      .to(table.scalar_type())
+      .reshape(shape);
+}
+
+Tensor plain_lookup_grad(const Tensor& ids, const Tensor& dy, int64_t num_rows, double scale,
+                         int64_t padding) {
+  Tensor to = inside(ids, num_rows);
+  if (padding >= 0) to = to.masked_fill(to == padding, num_rows);
+  const Tensor vals = dy.reshape({-1, dy.size(-1)}).to(at::kFloat) * scale;
+  return at::zeros({num_rows + 1, vals.size(1)}, vals.options())
+      .index_add(0, to, vals)
+      .narrow(0, 0, num_rows)
+      .to(dy.scalar_type());
+}
+
 struct LookupGrad;
 
 struct Lookup : torch::autograd::Function<Lookup> {
@@ -202,8 +257,11 @@ struct LookupGrad : torch::autograd::Function<LookupGrad> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor ids = ctx->get_saved_variables()[0];
     const int64_t padding = ctx->saved_data["padding"].toInt();
-    Tensor out = Lookup::apply(grads[0], ids, ctx->saved_data["status"].toOptional<Tensor>(),
-                               ctx->saved_data["scale"].toDouble(), padding, false);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    Tensor out = plain(grads[0])
+                     ? Lookup::apply(grads[0], ids, ctx->saved_data["status"].toOptional<Tensor>(), scale,
+                                     padding, false)
+                     : plain_lookup(grads[0], ids, scale);
     if (padding >= 0) out = out.masked_fill((ids == padding).unsqueeze(-1), 0.0);
     return {out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -227,6 +285,8 @@ variable_list Lookup::backward(AutogradContext* ctx, variable_list grads) {
     vals = vals.index_select(0, which);
     if (scale != 1.0) vals = vals * scale;
     dw = at::sparse_coo_tensor(flat.unsqueeze(0), vals, {rows, vals.size(1)});
+  } else if (!plain(grads[0])) {
+    dw = plain_lookup_grad(ids, grads[0], rows, scale, padding);
   } else if (at::GradMode::is_enabled()) {
     dw = LookupGrad::apply(grads[0], ids, status, rows, scale, padding);
   } else {
@@ -244,6 +304,7 @@ Tensor flag_of(const MaybeTensor& status, const Tensor& like) {
 
 Tensor embedding_rows_grad(const Tensor& ids, const Tensor& dy, int64_t num_rows, double scale,
                            std::optional<int64_t> padding, const MaybeTensor& status) {
+  require_plain(dy, ids, status);
   REFUSE_VALUE(dy.dim() < 1 || dy.sizes().slice(0, dy.dim() - 1) != ids.sizes(), "dy ", dy.sizes(),
                " does not belong to ids ", ids.sizes());
   REFUSE_VALUE(padding && (*padding < 0 || *padding >= num_rows), "padding_idx ", *padding,
@@ -259,6 +320,7 @@ Tensor embedding_rows_grad(const Tensor& ids, const Tensor& dy, int64_t num_rows
 
 Tensor embedding_rows(const Tensor& weight, const Tensor& ids, double scale,
                       std::optional<int64_t> padding, bool sparse, const MaybeTensor& status) {
+  require_plain(weight, ids, status);
   REFUSE_VALUE(weight.dim() != 2, "table must be [rows, dim], not ", weight.sizes());
   REFUSE_VALUE(padding && (*padding < 0 || *padding >= weight.size(0)), "padding_idx ", *padding,
                " is no row of the table");
@@ -306,6 +368,7 @@ struct Norm : torch::autograd::Function<Norm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &b = s[2], &stats = s[3];
+    require_plain(grads[0]);
     const int64_t dim = x.size(-1);
     const Rows r = rows_view(x, dim), g = rows_view(grads[0], dim);
     const int64_t m = r.t.size(0);
@@ -326,6 +389,7 @@ struct Norm : torch::autograd::Function<Norm> {
 };
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+  require_plain(x, weight, bias);
   REFUSE_VALUE(!(eps >= 0), "eps must not be negative, not ", eps);
   element_type(x, "x");
   REFUSE_VALUE(x.dim() < 1 || x.size(-1) < 1, "x must have a last dimension to normalise, not ",
@@ -444,6 +508,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto s = ctx->get_saved_variables();
     const int64_t want = wanted(ctx, ctx->saved_data["there"].toInt());
     std::array<Tensor, 5> d;
+    require_plain(grads[0]);
     if (want & 7)
       d = layer_backward(grads[0], s[0], s[1], Tensor(), s[2], Tensor(),
                          ctx->saved_data["act"].toInt(), (want & 3) | (want & 4) << 1);
@@ -465,6 +530,7 @@ struct Gated : torch::autograd::Function<Gated> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
+    require_plain(grads[0]);
     const auto d = layer_backward(grads[0], s[0], s[1], s[2], s[3], s[4],
                                   ctx->saved_data["act"].toInt(),
                                   wanted(ctx, ctx->saved_data["there"].toInt()));
@@ -474,6 +540,7 @@ struct Gated : torch::autograd::Function<Gated> {
 
 Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias,
               int64_t act, const MaybeTensor& residual) {
+  require_plain(x, weight, bias, residual);
   check_layer(x, weight);
   const Tensor w = param(weight, x, weight.sizes(), "weight");
   const Tensor b = param(bias, x, {weight.size(0)}, "bias"), r = given(residual);
@@ -494,6 +561,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias,
 Tensor gated_linear(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
                     const MaybeTensor& gate_bias, const MaybeTensor& up_bias,
                     int64_t act) {
+  require_plain(x, gate_weight, up_weight, gate_bias, up_bias);
   REFUSE_VALUE(gate_bias.has_value() != up_bias.has_value(), "gate_bias and up_bias: both or none");
   check_layer(x, gate_weight);
   const Tensor w = param(gate_weight, x, gate_weight.sizes(), "gate_weight");
@@ -525,6 +593,7 @@ PYBIND11_MODULE(_head_autograd, m) {
   m.def("layer_norm", &layer_norm, Unlocked());
   m.def("linear", &linear, Unlocked());
   m.def("gated_linear", &gated_linear, Unlocked());
+  m.def("plain", &plain);
   m.def("rows_view", [](const Tensor& t, int64_t width) {
     const Rows r = rows_view(t, width);
     return std::make_pair(r.t, r.ld);

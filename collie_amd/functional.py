@@ -6,7 +6,10 @@ residual, and the gated layer.  ``collie_amd.layers`` has them as modules.
 Inputs are float32, bfloat16 or float16 (all of one call alike; under ``torch.autocast`` the caller
 casts); sums, statistics and activations are computed in float32 and every result is rounded once.
 Gradients are summed in a fixed order: equal calls give equal bits.  Layers other than the embedding
-rows can be differentiated once.  There is no CPU fallback.
+rows can be differentiated once.  There is no CPU fallback.  What torch records or transforms by its
+own calls does not see these: tensors under ``vmap``, ``torch.func`` or ``torch.jit.trace``, fake
+tensors and forward-mode tangents are refused (the tables of ``collie_amd.layers``, called as modules,
+then do what ``torch.nn.Embedding`` does).
 
 Everything is launched on the current stream of the inputs' device and can be captured into a graph.
 As with any torch operation, drop eager results that depend on the same leaves before a backward pass

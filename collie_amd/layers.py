@@ -19,15 +19,30 @@ from collie_amd import _lib, functional
 
 class _Table(torch.nn.Embedding):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
-        # what the kernels do not take (other devices and types, empty tables, renormalised rows,
-        # gradients divided by counts) stays torch's
-        if (not self.weight.is_cuda or self.weight.numel() == 0
-                or self.weight.dtype not in _lib.ELEMENT_TYPES
-                or not input.is_cuda or input.dtype not in (torch.int32, torch.int64)
-                or self.max_norm is not None or self.scale_grad_by_freq):
-            return super().forward(input)
-        return functional.embedding_rows(self.weight, input, padding_idx=self.padding_idx,
-                                         sparse=self.sparse)
+        if torch.jit.is_scripting():        # (the other branch is not compiled then)
+            return torch.nn.functional.embedding(
+                input, self.weight, self.padding_idx, self.max_norm, self.norm_type,
+                self.scale_grad_by_freq, self.sparse)
+        else:
+            if not self._kernels_take(input):
+                return super().forward(input)
+            return functional.embedding_rows(self.weight, input, padding_idx=self.padding_idx,
+                                             sparse=self.sparse)
+
+    @torch.jit.unused
+    def _kernels_take(self, input) -> bool:
+        # What the kernels do not take stays torch's: other devices and types, empty tables,
+        # renormalised rows, gradients divided by counts; and calls that stand for others (recorded,
+        # compiled or transformed ones, tensors with forward-mode tangents).
+        if (torch.compiler.is_compiling() or torch.jit.is_tracing()
+                or torch.overrides.has_torch_function((input, self.weight))):
+            return False
+        return (self.weight.is_cuda and self.weight.numel() > 0
+                and self.weight.dtype in _lib.ELEMENT_TYPES
+                and input.is_cuda and input.dtype in (torch.int32, torch.int64)
+                and self.max_norm is None and not self.scale_grad_by_freq
+                and _lib.load_autograd().plain(self.weight)
+                and _lib.load_autograd().plain(input))
 
 
 class ScaledEmbedding(_Table):

@@ -24,3 +24,96 @@ def test_sparse_gradient_leaves_out_ids_outside_the_table(bad, padding):
     want = [r for r in ids.reshape(-1).tolist() if 0 <= r < 6 and r != padding]
     assert rows == want and g._values().shape == (len(want), 4)
     assert (g._values() == 0.5).all()       # exact: one factor of one half
+
+
+# ---- the tables as modules under torch's transforms ------------------------------------------------
+def _table(rows=9, dim=5, **kw):
+    from collie_amd import layers
+    torch.manual_seed(3)
+    t = layers.ScaledEmbedding(rows, dim, **kw).to(DEV)
+    with torch.no_grad():
+        t.weight.normal_()
+    return t
+
+
+IDS = torch.tensor([[1, 8, 0], [8, 8, 3]])
+
+
+@pytest.mark.parametrize('frozen', [True, False])
+@pytest.mark.parametrize('grad_mode', [True, False])
+def test_tables_carry_a_forward_mode_tangent(frozen, grad_mode):
+    import torch.autograd.forward_ad as fw
+    t = _table()
+    t.weight.requires_grad_(not frozen)
+    ids, tangent = IDS.to(DEV), torch.randn(9, 5).to(DEV)
+    with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = fw.make_dual(t.weight, tangent)
+        y, dy = fw.unpack_dual(torch.func.functional_call(t, {'weight': dual}, (ids,)))
+    assert torch.equal(y, t.weight[ids]) and torch.equal(dy, tangent[ids])
+
+
+@pytest.mark.parametrize('how', ['script', 'trace', 'vmap', 'func_grad', 'jvp', 'compile'])
+def test_tables_can_be_recorded_and_transformed(how):
+    t = _table()
+    t.weight.requires_grad_(False)
+    ids = IDS.to(DEV)
+    want = t.weight[ids]
+    if how == 'script':
+        got = torch.jit.script(t)(ids)
+    elif how == 'trace':
+        traced = torch.jit.trace(t, (ids,))
+        torch.empty(1 << 20, device=DEV).fill_(7.0)     # what a recorded allocation might find
+        got = traced(ids)
+    elif how == 'vmap':
+        got = torch.vmap(t)(ids)
+    elif how == 'compile':
+        got = torch.compile(t, backend='eager', fullgraph=True)(ids)
+    else:
+        f = lambda w: torch.func.functional_call(t, {'weight': w}, (ids,))      # noqa: E731
+        if how == 'func_grad':
+            got = torch.func.grad(lambda w: f(w).sum())(t.weight)
+            want = torch.bincount(ids.reshape(-1), minlength=9)[:, None].expand(9, 5).float()
+        else:
+            got, tangent = torch.func.jvp(f, (t.weight,), (2 * t.weight,))
+            assert torch.equal(tangent, 2 * want)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize('padding', [None, 3])
+def test_gradients_of_a_table_under_transforms(padding):
+    """Batched gradients, gradients of gradients of them, and a tangent that comes from elsewhere, as
+    torch.nn.Embedding has them (whole numbers: exact)."""
+    import torch.autograd.forward_ad as fw
+    own, ref = _table(padding_idx=padding), torch.nn.Embedding(9, 5, padding_idx=padding).to(DEV)
+    ids = IDS.to(DEV)
+    with torch.no_grad():
+        ref.weight.copy_(own.weight.round())
+        own.weight.copy_(ref.weight)
+    g = torch.Generator().manual_seed(4)
+    dys = torch.randint(-3, 4, (4, 2, 3, 5), generator=g).float().to(DEV)
+    got = {}
+    for name, t in (('own', own), ('ref', ref)):
+        y = t(ids)
+        (rows,) = torch.autograd.grad(y, [t.weight], dys, is_grads_batched=True, retain_graph=True)
+        out = [rows]
+        dy = dys[0].clone().requires_grad_()
+        (grad,) = torch.autograd.grad(y, [t.weight], dy, create_graph=True)
+        (back,) = torch.autograd.grad(grad, [dy], torch.stack([torch.ones_like(grad), grad.detach()]),
+                                      is_grads_batched=True)
+        out.append(back)
+        with fw.dual_level():
+            other = fw.make_dual(dys[1], dys[2])
+            (grad,) = torch.autograd.grad((t(ids) * other).sum(), [t.weight])
+            out += list(fw.unpack_dual(grad))
+        got[name] = out
+    for a, b in zip(got['own'], got['ref']):
+        assert b is not None and torch.equal(a, b)
+
+
+def test_layers_refuse_gradients_that_stand_for_others():
+    from collie_amd import _lib, functional as F
+    x, w = torch.ones(3, 4, device=DEV, requires_grad=True), torch.ones(5, 4, device=DEV)
+    for y in (F.linear(x, w, activation='silu'), F.gated_linear(x, w, w), F.layer_norm(x)):
+        with pytest.raises(RuntimeError, match='vmap, torch.func or torch.jit.trace'):
+            torch.autograd.grad(y, [x], torch.ones(2, *y.shape, device=DEV), is_grads_batched=True)
+    assert issubclass(_lib.CollieHipError, RuntimeError)
