@@ -4,7 +4,8 @@ Parameter containers of the MF model (reference: ``collie/model/base/layers.py``
 The tables are ``torch.nn.Embedding`` subclasses, so that ``state_dict()`` keys, shapes, the
 ``sparse`` flag and the initial distributions are those of the reference.  The fused paths look rows
 up inside their own kernels, straight from ``.weight``; a table that is called as a module takes
-``functional.embedding_rows`` on a HIP device.
+``functional.embedding_rows`` on a HIP device, where an id outside the table gives a row of zeros and
+an ``IndexError`` at the next ``check_status()``.
 
 ``LayerNorm``, ``Linear`` and ``GatedLinear`` are the layers of a deeper ranking head
 (``collie_amd.functional``) with the parameter names and the initialisation of their ``torch.nn``
@@ -17,7 +18,10 @@ import torch
 from collie_amd import _lib, functional
 
 
-class _Table(torch.nn.Embedding):
+class Table(torch.nn.Embedding):
+    # int32 [1] on the table's device once it has been called there: bit 0 says that an id was outside
+    _status = None
+
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         if torch.jit.is_scripting():        # (the other branch is not compiled then)
             return torch.nn.functional.embedding(
@@ -27,7 +31,24 @@ class _Table(torch.nn.Embedding):
             if not self._kernels_take(input):
                 return super().forward(input)
             return functional.embedding_rows(self.weight, input, padding_idx=self.padding_idx,
-                                             sparse=self.sparse)
+                                             sparse=self.sparse, status=self._status_flag())
+
+    @torch.jit.unused
+    def _status_flag(self):
+        if self._status is None or self._status.device != self.weight.device:
+            if torch.cuda.is_current_stream_capturing():
+                return None     # memory of the graph, which would clear it with every replay
+            self._status = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
+        return self._status
+
+    @torch.jit.unused
+    def check_status(self):
+        """Raise ``IndexError`` if a call since the last check had an id outside the table (syncs).
+        On a HIP device such an id gives a row of zeros and takes no gradient; the models look here
+        where they look at the flag of their own kernels (``MatrixFactorizationModel.check_status``)."""
+        if self._status is not None and int(self._status.item()) & 1:
+            self._status.zero_()
+            raise IndexError('index out of range in self: an id is outside the table')
 
     @torch.jit.unused
     def _kernels_take(self, input) -> bool:
@@ -45,14 +66,14 @@ class _Table(torch.nn.Embedding):
                 and _lib.load_autograd().plain(input))
 
 
-class ScaledEmbedding(_Table):
+class ScaledEmbedding(Table):
     """N(0, (1 / (2.5 * embedding_dim))^2) initialisation (``layers.py:6-10``)."""
 
     def reset_parameters(self) -> None:
         self.weight.data.normal_(0, 1.0 / (self.embedding_dim * 2.5))
 
 
-class ZeroEmbedding(_Table):
+class ZeroEmbedding(Table):
     """All-zero initialisation (``layers.py:13-17``)."""
 
     def reset_parameters(self) -> None:

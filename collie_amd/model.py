@@ -32,7 +32,7 @@ from torch.optim.lr_scheduler import ReduceLROnPlateau
 from collie_amd import _lib, functional, loss as loss_mod, ops
 from collie_amd.interactions import (ApproximateNegativeSamplingInteractionsDataLoader,
                                      Interactions, InteractionsDataLoader)
-from collie_amd.layers import ScaledEmbedding, ZeroEmbedding
+from collie_amd.layers import ScaledEmbedding, Table, ZeroEmbedding
 from collie_amd.optim import FUSED_OPTIMIZERS
 
 
@@ -447,6 +447,9 @@ class MatrixFactorizationModel(nn.Module):
         if self._status is not None and int(self._status.item()) & 1:
             self._status.zero_()
             raise IndexError('index out of range in self: a user or item id is outside the tables')
+        for module in self.modules():       # tables that a subclass has called as modules
+            if isinstance(module, Table):
+                module.check_status()
 
     def check_anomaly(self):
         """``detect_anomaly`` on the fused route (``trainer.py:333``): raise ``RuntimeError`` if a
