@@ -279,7 +279,10 @@ dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', l
         for i, layer in enumerate(self.combined_layers):
             nn.init.xavier_normal_(layer.weight)
             self.add_module('combined_layer_{}'.format(i), layer)
-        # (hyper-parameters saved before there were blocks do not name them)
+        # (hyper-parameters saved before there were blocks do not name them; a model that becomes the
+        # copy of another, load_from_hybrid_model, may have had more)
+        for name in [n for n in self._modules if n.startswith('combined_block_')]:
+            del self._modules[name]
         self.combined_blocks = []
         for i in range(hp.get('combined_blocks') or 0):
             if len(self.combined_layers) < 2:
@@ -345,6 +348,7 @@ dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', l
         """``hybrid_pretrained_matrix_factorization.py:536-555``."""
         for key, value in hybrid_model.hparams.items():
             self.hparams[key] = value
+        self.hparams['combined_blocks'] = hybrid_model.hparams.get('combined_blocks') or 0
         self.hparams['load_model_path'] = 'copied'      # rebuild layers from hparams, not a trained model
         self._setup_model()
         self.hparams['load_model_path'] = None
