@@ -340,19 +340,19 @@ int32_t norm_param_type(const Tensor& w, const Tensor& b, const Tensor& x) {
   return element_type(w.defined() ? w : b.defined() ? b : x, "weight");
 }
 
-// y, and mean and rstd [2, rows] with `keep`
+// y, and mean (two parts) and rstd [3, rows] with `keep`
 std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps,
                                        bool keep) {
   const int64_t dim = x.size(-1);
   const Rows r = rows_view(x, dim);
   const int64_t m = r.t.size(0);
   Tensor y = at::empty(x.sizes(), x.options());
-  Tensor stats = keep ? at::empty({2, m}, x.options().dtype(at::kFloat)) : Tensor();
+  Tensor stats = keep ? at::empty({3, m}, x.options().dtype(at::kFloat)) : Tensor();
   float* mean = static_cast<float*>(at_or_null(stats));
   c10::DeviceGuard guard(x.device());
   check(collie_layer_norm_forward(r.t.data_ptr(), r.ld, element_type(x, "x"), m, dim, at_or_null(w),
                                   at_or_null(b), norm_param_type(w, b, x), eps, y.data_ptr(), mean,
-                                  mean ? mean + m : nullptr, stream_of(x)),
+                                  mean ? mean + 2 * m : nullptr, stream_of(x)),
         "collie_layer_norm_forward");
   return {y, stats};
 }
@@ -380,7 +380,7 @@ struct Norm : torch::autograd::Function<Norm> {
     const float* mean = stats.data_ptr<float>();
     c10::DeviceGuard guard(x.device());
     check(collie_layer_norm_backward(g.t.data_ptr(), g.ld, r.t.data_ptr(), r.ld, element_type(x, "x"),
-                                     m, dim, at_or_null(w), norm_param_type(w, b, x), mean, mean + m,
+                                     m, dim, at_or_null(w), norm_param_type(w, b, x), mean, mean + 2 * m,
                                      at_or_null(dx), at_or_null(dw), at_or_null(db), ws.data_ptr(),
                                      ws.numel(), stream_of(x)),
           "collie_layer_norm_backward");

@@ -23,7 +23,7 @@ struct NormParams {
   const void* w;     // NULL: ones
   const void* b;     // NULL: zeros
   void* y;           // backward: dx (NULL: not wanted)
-  float* mean;
+  float* mean;       // [2, rows]: the mean, and what is left of it after rounding
   float* rstd;
   float* partial;    // backward: [workgroups, 2, dim] (NULL: not wanted)
   void *dw, *db;     // backward with one workgroup: the sums themselves, of the parameters' type
@@ -68,6 +68,20 @@ __device__ __forceinline__ void row_sums(float (&s)[N]) {
   }
 }
 
+// mean of squares about a point that is `off` from the mean -> variance
+__device__ __forceinline__ float variance(float squares, float off) {
+  const float v = fmaf(-off, off, squares);
+  return v < 0.0f ? 0.0f : v;  // (NaN stays)
+}
+
+__device__ __forceinline__ void keep_stats(const NormParams& p, int64_t row, float first, float off,
+                                           float rstd) {
+  const float mean = first + off;
+  p.mean[row] = mean;
+  p.mean[p.rows + row] = off - (mean - first);
+  p.rstd[row] = rstd;
+}
+
 // lane `sub` of a row owns the packs sub, sub + TPR, ...; WHOLE: dim is a whole number of packs
 template <typename T, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void norm_fwd_kernel(const NormParams p) {
@@ -98,29 +112,30 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_kernel(const NormParams p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] += v[i][j];
     row_sums<TPR>(s);
-    const float mean = s[0] * inv;
-    s[0] = 0.0f;
+    const float first = s[0] * inv;
+    // what the mean was rounded by is the mean of what is left: a constant row has no variance then,
+    // however large its value (1e6 over 49 columns: the sum times 1 / 49 is 0.06 off)
+    float c[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = j < left[i] ? v[i][j] - mean : 0.0f;
-        s[0] = fmaf(v[i][j], v[i][j], s[0]);
+        v[i][j] = j < left[i] ? v[i][j] - first : 0.0f;
+        c[0] += v[i][j];
+        c[1] = fmaf(v[i][j], v[i][j], c[1]);
       }
-    row_sums<TPR>(s);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + p.eps);
+    row_sums<TPR>(c);
+    const float off = c[0] * inv;
+    const float rstd = 1.0f / sqrtf(variance(c[1] * inv, off) + p.eps);
     if (!live) continue;
     T* y = static_cast<T*>(p.y) + row * p.dim;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
+      for (int j = 0; j < V; ++j) v[i][j] = fmaf((v[i][j] - off) * rstd, w[i][j], b[i][j]);
       if (left[i] > 0) store_pack<T, V>(y + col[i], left[i], v[i], p.stream);
     }
-    if (sub == 0 && p.mean) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
+    if (sub == 0 && p.mean) keep_stats(p, row, first, off, rstd);
   }
 }
 
@@ -148,7 +163,7 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const NormParams p) {
     const int64_t at = live ? row : 0;
     const T* x = static_cast<const T*>(p.x) + at * p.x_ld;
     const T* dy = static_cast<const T*>(p.dy) + at * p.dy_ld;
-    const float mean = p.mean[at], rstd = p.rstd[at];
+    const float mean = p.mean[at], low = p.mean[p.rows + at], rstd = p.rstd[at];
     float h[NV][V], g[NV][V], s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -159,7 +174,7 @@ __global__ __launch_bounds__(kBlock) void norm_bwd_kernel(const NormParams p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[i][j] = j < left[i] ? (h[i][j] - mean) * rstd : 0.0f;
+        h[i][j] = j < left[i] ? (h[i][j] - mean - low) * rstd : 0.0f;
         if (live) {
           dw[i][j] = fmaf(g[i][j], h[i][j], dw[i][j]);
           db[i][j] += g[i][j];
@@ -230,18 +245,20 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_wide_kernel(const NormParams 
       for (int j = 0; j < V; ++j) s[0] += v[j];
     }
     row_sums<kBlock>(s);
-    const float mean = s[0] * inv;
-    s[0] = 0.0f;
+    const float first = s[0] * inv;
+    float t[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x * V; c < p.dim; c += kBlock * V) {
       load_pack<T, V>(x + c, p.dim - c, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = c + j < p.dim ? v[j] - mean : 0.0f;
-        s[0] = fmaf(d, d, s[0]);
+        const float d = c + j < p.dim ? v[j] - first : 0.0f;
+        t[0] += d;
+        t[1] = fmaf(d, d, t[1]);
       }
     }
-    row_sums<kBlock>(s);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + p.eps);
+    row_sums<kBlock>(t);
+    const float off = t[0] * inv;
+    const float rstd = 1.0f / sqrtf(variance(t[1] * inv, off) + p.eps);
     T* y = static_cast<T*>(p.y) + row * p.dim;
     for (int c = threadIdx.x * V; c < p.dim; c += kBlock * V) {
       float w[V], b[V];
@@ -249,13 +266,10 @@ __global__ __launch_bounds__(kBlock) void norm_fwd_wide_kernel(const NormParams 
       load_param<T, V>(p.w, p.w_f32, c, p.dim - c, 1.0f, w);
       load_param<T, V>(p.b, p.w_f32, c, p.dim - c, 0.0f, b);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * rstd, w[j], b[j]);
+      for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - first - off) * rstd, w[j], b[j]);
       store_pack<T, V>(y + c, p.dim - c, v);
     }
-    if (threadIdx.x == 0 && p.mean) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
+    if (threadIdx.x == 0 && p.mean) keep_stats(p, row, first, off, rstd);
   }
 }
 
@@ -266,7 +280,7 @@ __global__ __launch_bounds__(kBlock) void norm_dx_wide_kernel(const NormParams p
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
     const T* dy = static_cast<const T*>(p.dy) + row * p.dy_ld;
-    const float mean = p.mean[row], rstd = p.rstd[row];
+    const float mean = p.mean[row], low = p.mean[p.rows + row], rstd = p.rstd[row];
     float h[V], g[V], w[V], s[2] = {0.0f, 0.0f};
     auto load = [&](int c) {
       load_pack<T, V>(x + c, p.dim - c, h);
@@ -274,7 +288,7 @@ __global__ __launch_bounds__(kBlock) void norm_dx_wide_kernel(const NormParams p
       load_param<T, V>(p.w, p.w_f32, c, p.dim - c, 1.0f, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[j] = c + j < p.dim ? (h[j] - mean) * rstd : 0.0f;
+        h[j] = c + j < p.dim ? (h[j] - mean - low) * rstd : 0.0f;
         g[j] *= w[j];
       }
     };
@@ -307,7 +321,7 @@ __global__ __launch_bounds__(kBlock) void norm_dw_wide_kernel(const NormParams p
   for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float g = static_cast<float>(static_cast<const T*>(p.dy)[row * p.dy_ld + c]);
     const float x = static_cast<float>(static_cast<const T*>(p.x)[row * p.x_ld + c]);
-    dw = fmaf(g, (x - p.mean[row]) * p.rstd[row], dw);
+    dw = fmaf(g, (x - p.mean[row] - p.mean[p.rows + row]) * p.rstd[row], dw);
     db += g;
   }
   float* out = p.partial + static_cast<int64_t>(blockIdx.y) * 2 * p.dim;

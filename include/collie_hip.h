@@ -830,8 +830,8 @@ int collie_embedding_rows_grad(const void* ids, int32_t ids_dtype, int64_t n, co
                                size_t workspace_bytes, int32_t* status, collie_stream_t stream);
 
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (biased variance).
- * weight / bias (NULL: ones / zeros) are float32 or of x's type (w_dtype); mean / rstd [rows] are
- * written for the backward pass (NULL: not wanted). */
+ * weight / bias (NULL: ones / zeros) are float32 or of x's type (w_dtype); mean [2, rows] (rounded, and
+ * what is left of it) / rstd [rows] are written for the backward pass (NULL: not wanted). */
 int collie_layer_norm_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t rows, int32_t dim,
                               const void* weight, const void* bias, int32_t w_dtype, float eps,
                               void* y, float* mean, float* rstd, collie_stream_t stream);

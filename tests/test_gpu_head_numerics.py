@@ -1,0 +1,76 @@
+"""
+GPU tests (``-m gpu``) of the ranking-head operators where their numbers are hard: large constants under
+a layer norm, tails of activations, and intermediate values at the ends of a type's range.
+"""
+import pytest
+import torch
+
+import head_bounds as hb
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda:0')
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+F = hb.F
+
+
+# ---- layer norm of rows that lie far from zero -----------------------------------------------------
+def chain(dim):
+    """Roundings of a sum over a row: values that one lane adds, then a tree (see hb.layer_norm)."""
+    return (min(dim, 64) if dim <= 8192 else dim // 256 + 8) + 12
+
+
+DIMS = [7, 30, 109, 255, 600, 1023, 3001, 8193, 20011]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('dim', DIMS)
+def test_layer_norm_of_large_constant_rows(dim, dtype):
+    """The mean c (1 + d) is off by |d| <= chain F, what is left of a value, c d, is exact, and so is its
+    mean but for chain + 2 roundings: at most c chain (chain + 2) F^2 stays, over sqrt(eps)."""
+    from collie_amd import functional
+    c = {torch.float32: 1e6, torch.bfloat16: 999424.0, torch.float16: 60000.0}[dtype]
+    x = torch.tensor([c, -c, c / 4]).to(dtype)[:, None].expand(3, dim).contiguous()
+    leaf = x.to(DEV).requires_grad_()
+    y = functional.layer_norm(leaf)
+    k = chain(dim)
+    assert y.detach().abs().max().item() <= c * k * (k + 2) * F * F / 1e-5 ** 0.5
+    # the gradient of a row without variance is (dy - mean(dy)) / sqrt(eps): its inner product with the
+    # row's values, all alike, is part of what is rounded
+    dy = torch.ones_like(y)
+    (dx,) = torch.autograd.grad(y, [leaf], dy)
+    assert dx.abs().max().item() <= 4 * k * F / 1e-5 ** 0.5
+
+
+@pytest.mark.parametrize('dim', DIMS)
+def test_layer_norm_of_rows_with_a_large_mean(dim):
+    """Whole numbers around 1e6: differences from the mean of their first rounding are exact, so the
+    result and its gradients keep float32's accuracy relative to the largest of the row."""
+    from collie_amd import functional
+    g = torch.Generator().manual_seed(dim)
+    x = 1e6 + torch.randint(-3, 4, (5, dim), generator=g).float()
+    w, dy = torch.randn(dim, generator=g), torch.randn(5, dim, generator=g)
+    leaves = [x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()]
+    y = functional.layer_norm(*leaves)
+    dx, dw = torch.autograd.grad(y, leaves, dy.to(DEV))
+    x, w, dy = x.double(), w.double(), dy.double()
+    xc = x - x.mean(1, keepdim=True)
+    var = (xc * xc).mean(1, keepdim=True)
+    r = (var + 1e-5).rsqrt()
+    h = xc * r
+    k = chain(dim)
+    # relative error of rstd: half of what k + 6 roundings do to the squares, which contain the square of
+    # the first mean's error (k F 1e6 at most) until that is taken out again
+    er = (k + 6) * F * (1 + (k * F * 1e6) ** 2 / var)
+    # (v - off): off is off by k + 2 roundings of the mean of |v|, v by nothing
+    eh = (k + 8) * F * (h.abs().mean(1, keepdim=True) + h.abs()) + h.abs() * er
+    room = eh * w.abs() + 2 * F * (h * w).abs() + F * (h * w).abs()
+    hb.check(y.detach(), h * w, room, torch.float32)
+    gr = dy * w
+    m1, m2 = gr.mean(1, keepdim=True), (gr * h).mean(1, keepdim=True)
+    e1 = (k + 4) * F * gr.abs().mean(1, keepdim=True)
+    e2 = (gr.abs() * eh).mean(1, keepdim=True) + (k + 6) * F * (gr * h).abs().mean(1, keepdim=True)
+    inner = gr - m1 - h * m2
+    ei = F * gr.abs() + e1 + h.abs() * e2 + eh * (m2.abs() + e2) + 4 * F * (gr.abs() + m1.abs()
+                                                                             + (h * m2).abs())
+    hb.check(dx, r * inner, r * (ei + (er + 2 * F) * (inner.abs() + ei)) * 1.01, torch.float32)
+    hb.check(dw, (dy * h).sum(0), (dy.abs() * eh).sum(0) + 25 * F * (dy * h).abs().sum(0), torch.float32)
