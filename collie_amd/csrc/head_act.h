@@ -7,33 +7,41 @@ namespace collie {
 
 constexpr float kLeakySlope = 0.01f;  // F.leaky_relu's default, as in the hybrid head
 
-// 1 / (1 + exp(-z)) to about two steps of float32: 2^t with t = -z log2(e) in two parts (the product
-// and what it was rounded by), and the reciprocal instruction.  The library's expf and division took
-// a third of the gated layer's forward pass (16,384 x 2,048 x 5,504: 988 us with them).
-__device__ __forceinline__ float fast_exp(float x) {
+// exp(x + low), x of magnitude below 100 and low a part below its last bit: 2^t with t = x log2(e) in two
+// parts (the product and what it was rounded by).  The library's expf and division took a third of the
+// gated layer's forward pass (16,384 x 2,048 x 5,504: 988 us with them).
+__device__ __forceinline__ float fast_exp(float x, float low = 0.0f) {
   const float t = x * 1.44269504f;
-  const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+  const float rest = fmaf(x, 1.44269504f, -t) + fmaf(x, 1.92596299e-8f, low * 1.44269504f);
   const float e = __builtin_amdgcn_exp2f(t);
   // beyond, e is at an end of the range (infinite times a correction would be NaN)
   return fabsf(t) < 126.0f ? fmaf(e, rest * 0.693147181f, e) : e;
 }
+// 1 / (1 + exp(-z)) to about two steps of float32
 __device__ __forceinline__ float fast_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z));
 }
 
-// Phi(z), the normal distribution function, and exp(-z^2 / 2) with it: Abramowitz and Stegun, Handbook
-// of Mathematical Functions, 7.1.26 (erfc to 1.5e-7), without a branch; the side of small values is
-// computed as such.  The library's erff cost the forward pass of 720,896 x 256 x 128 (float32) 100 us
-// of 580.
+// Phi(z), the normal distribution function, to eight half steps of float32 of its value on either side,
+// and exp(-z^2 / 2) with it, without a branch: Phi(-|z|) = t P(t) exp(-z^2 / 2), t = 1 / (1 + 0.35 |z|).
+// P is the polynomial of degree 8 with the least relative error (3.2e-8) against
+// erfc(x) exp(x^2) / (2 t), x = |z| / sqrt(2), over |z| <= 14, found by Remez's exchange from erfc in
+// 40 digits.  What z^2 is rounded by would be 50 half steps of the exponential at |z| = 10, so it goes in
+// as the low part.  The library's erff cost the forward pass of 720,896 x 256 x 128 (float32) 100 us of
+// 580.
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-  float p = fmaf(t, 1.061405429f, -1.453152027f);
-  p = fmaf(t, p, 1.421413741f);
-  p = fmaf(t, p, -0.284496736f);
-  p = fmaf(t, p, 0.254829592f);
-  e = fast_exp(-x * x);
-  const float tail = 0.5f * p * t * e;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(z), 1.0f));
+  float p = fmaf(t, -0.0291459142f, 0.143971623f);
+  p = fmaf(t, p, -0.255714108f);
+  p = fmaf(t, p, 0.159174003f);
+  p = fmaf(t, p, -0.0231097335f);
+  p = fmaf(t, p, 0.105507964f);
+  p = fmaf(t, p, 0.119832877f);
+  p = fmaf(t, p, 0.139861868f);
+  p = fmaf(t, p, 0.139621404f);
+  const float h = z * z;
+  e = fast_exp(-0.5f * h, -0.5f * fmaf(z, z, -h));
+  const float tail = p * t * e;
   return z < 0.0f ? tail : 1.0f - tail;
 }
 

@@ -74,3 +74,23 @@ def test_layer_norm_of_rows_with_a_large_mean(dim):
                                                                              + (h * m2).abs())
     hb.check(dx, r * inner, r * (ei + (er + 2 * F) * (inner.abs() + ei)) * 1.01, torch.float32)
     hb.check(dw, (dy * h).sum(0), (dy.abs() * eh).sum(0) + 25 * F * (dy * h).abs().sum(0), torch.float32)
+
+
+# ---- activations far from zero ---------------------------------------------------------------------
+def test_gelu_keeps_the_digits_of_its_tail():
+    """z Phi(z) and its slope in float32, one column, weight one.  Phi: the exponential and its two parts
+    (4 F with the instruction), the polynomial (its own 1 F, 4 F of rounding), the reciprocal (2 F, which
+    t times the polynomial feels at most twice), three products; with the product by z 16 F at most."""
+    from collie_amd import functional
+    z = torch.cat([torch.linspace(-12.4, 9.0, 30001), torch.tensor([0.0, -0.0, 1e-30, -1e-30])])
+    z = z.reshape(-1, 1)
+    x, w = z.to(DEV).requires_grad_(), torch.ones(1, 1, device=DEV)
+    y = functional.linear(x, w, activation='gelu')
+    (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    z = z.double()
+    phi, pdf = torch.special.log_ndtr(z).exp(), torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    tiny = 2.0 ** -126                      # (z = 1e-30 is kept, its square is not)
+    assert ((y.double().cpu() - z * phi).abs() <= 16 * F * (z * phi).abs() + tiny).all()
+    # Phi + z pdf(z): both to 16 F, their sum, dz and the product (four dropped parts) round once each
+    room = 20 * F * (phi + (z * pdf).abs()) + tiny
+    assert ((dx.double().cpu() - (phi + z * pdf)).abs() <= room).all()
