@@ -125,19 +125,17 @@ __device__ __forceinline__ void act_slopes(int act, float (&v)[N], float (&d)[N]
   }
 }
 
-// A pre-activation kept for the backward pass.  The linear layer keeps it in its own type: f' of it is
-// then off by half a step of that type times a slope of at most one, less than what dz is rounded by
-// anyway.  float16 ends at 65504, where every activation here has reached its end: a larger value is
-// kept as that one, because an infinity would turn z (1 - sigmoid(z)) into inf * 0.  The gated layer
-// keeps float32: its gradients are products of two kept values, and 16 bits of each put them 1.8
-// times as far from the float64 ones as one rounding of the result does (1.4 times with float32).
+// Pre-activations kept for the backward pass are float32, in the linear layer (where f' is smooth) and in
+// the gated one (whose gradients contain f, f' and u).  16 bits of z are not enough for f'(z): a relative
+// change d of z is one of d z f''(z) / f'(z), |z| times as much in a sigmoid's tail and without bound next
+// to the zero of silu's or gelu's slope.  Of relu and leaky_relu only the sign counts, so the linear layer
+// keeps their z in its own type, and what is positive as something positive.
+__host__ __device__ constexpr bool kept_in_float(int act) { return act >= COLLIE_ACT_SIGMOID; }
+
 template <typename T>
-__device__ __forceinline__ float kept(float z) {
-  return z;
-}
-template <>
-__device__ __forceinline__ float kept<f16_t>(float z) {
-  return fabsf(z) < INFINITY ? fminf(fmaxf(z, -65504.0f), 65504.0f) : z;
+__device__ __forceinline__ float kept_sign(float z) {
+  constexpr float least = std::is_same<T, f16_t>::value ? 6.10351562e-5f : 1.17549435e-38f;
+  return z > 0.0f && z < least ? least : z;
 }
 
 }  // namespace collie

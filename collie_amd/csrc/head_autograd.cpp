@@ -436,7 +436,8 @@ Forward layer_forward(const Tensor& x, const Tensor& w, const Tensor& w2, const 
     f.keep = at::empty({m, n_out}, x.options().dtype(at::kFloat));
     f.keep2 = at::empty({m, n_out}, x.options().dtype(at::kFloat));
   } else if (keep && act != COLLIE_ACT_IDENTITY) {
-    f.keep = at::empty({m, n_out}, x.options());
+    const bool sign_only = act == COLLIE_ACT_RELU || act == COLLIE_ACT_LEAKY_RELU;
+    f.keep = at::empty({m, n_out}, sign_only ? x.options() : x.options().dtype(at::kFloat));
   }
   const Tensor ws = scratch(collie_layer_forward_workspace_bytes(r.t.data_ptr(), r.ld, tag, m, n_in,
                                                                  w.data_ptr(), at_or_null(w2), n_out),

@@ -31,7 +31,7 @@ struct Gemm {
   const void *bias, *bias2;
   const void* residual;
   int64_t res_ld;
-  void *keep, *keep2;    // pre-activations for the backward pass [m, n], or NULL (gated: float32)
+  void *keep, *keep2;    // pre-activations for the backward pass [m, n], or NULL (see head_act.h)
   void *c, *c2;          // output [m, n]; with kEpiStore rows >= row_split are c2's, and of either
   int64_t row_split;     // only the first row_valid are wanted
   int64_t row_valid;
@@ -71,9 +71,11 @@ __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t c
       if constexpr (EPI == kEpiGated) {
         store_pack<float, W>(static_cast<float*>(g.keep) + at, left, v, g.stream);
         store_pack<float, W>(static_cast<float*>(g.keep2) + at, left, u, g.stream);
+      } else if (kept_in_float(g.act)) {
+        store_pack<float, W>(static_cast<float*>(g.keep) + at, left, v, g.stream);
       } else {
 #pragma unroll
-        for (int j = 0; j < W; ++j) t[j] = kept<T>(v[j]);
+        for (int j = 0; j < W; ++j) t[j] = kept_sign<T>(v[j]);
         store_pack<T, W>(static_cast<T*>(g.keep) + at, left, t, g.stream);
       }
     }

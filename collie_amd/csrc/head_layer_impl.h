@@ -21,7 +21,7 @@ constexpr int kBlock = 256;
 // ---- dz = dy f'(z) (linear), [dg | du] (gated), and the column sums for the bias gradients --------
 struct ActBwd {
   const void *dy;
-  const void *z, *u;       // kept pre-activations: of the rows' type (NULL: identity), gated: float32
+  const void *z, *u;       // kept pre-activations (head_act.h; NULL: identity)
   void* dz;                // [m, dz_ld]; NULL: only the column sums are wanted
   float* partial;          // [gridDim.y, pair * n]: column sums, or NULL
   void *db, *db2;          // gridDim.y = 1: the sums themselves (either may be NULL) instead
@@ -49,9 +49,11 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
       float dy[V], z[V], d[V], u[V];
       load_pack<T, V>(static_cast<const T*>(p.dy) + row * p.dy_ld + col, left, dy);
       if (p.z) {
-        using K = std::conditional_t<PAIR, float, T>;
-        load_pack<K, V>(static_cast<const K*>(p.z) + row * p.n + col, left, z);
-        if (PAIR) load_pack<K, V>(static_cast<const K*>(p.u) + row * p.n + col, left, u);
+        if (PAIR || kept_in_float(p.act))
+          load_pack<float, V>(static_cast<const float*>(p.z) + row * p.n + col, left, z);
+        else
+          load_pack<T, V>(static_cast<const T*>(p.z) + row * p.n + col, left, z);
+        if (PAIR) load_pack<float, V>(static_cast<const float*>(p.u) + row * p.n + col, left, u);
         act_slopes(p.act, z, d);
       }
 #pragma unroll
@@ -271,7 +273,8 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, bool pair, double out_bytes) {
   return best;
 }
 
-// what the forward pass stores per accumulator when the backward pass is to follow
+// what the forward pass stores per accumulator when the backward pass is to follow (the linear layer's
+// kept values in its own type: the workspace is asked for before the activation is known)
 template <typename T>
 double stored_bytes(bool pair) {
   return pair ? (sizeof(T) + 8.0) / 2 : 2.0 * sizeof(T);

@@ -865,8 +865,9 @@ size_t collie_layer_backward_workspace_bytes(const void* dy, int64_t dy_ld, cons
                                              int32_t n_out, int32_t act);
 
 /* y = act(x weight^T + bias) + residual ([m, n_out]); weight [n_out, n_in]; bias / residual may be
- * NULL.  keep [m, n_out] (NULL: not wanted) takes the pre-activations, in x's type (float16:
- * finite ones beyond +-65504 as that), for the backward pass. */
+ * NULL.  keep [m, n_out] (NULL: not wanted) takes the pre-activations for the backward pass: float32
+ * for sigmoid, silu and gelu; for relu and leaky_relu in x's type, where only the sign is kept to the
+ * last bit. */
 int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m, int32_t n_in,
                           const void* weight, const void* bias, int32_t n_out, int32_t act,
                           const void* residual, int64_t res_ld, void* keep, void* y,

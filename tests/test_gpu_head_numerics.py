@@ -94,3 +94,40 @@ def test_gelu_keeps_the_digits_of_its_tail():
     # Phi + z pdf(z): both to 16 F, their sum, dz and the product (four dropped parts) round once each
     room = 20 * F * (phi + (z * pdf).abs()) + tiny
     assert ((dx.double().cpu() - (phi + z * pdf)).abs() <= room).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES[1:])
+@pytest.mark.parametrize('kind', ['sigmoid', 'silu', 'gelu'])
+def test_slopes_are_those_of_the_unrounded_sums(kind, dtype):
+    """z = a + b with b far below a's last bits, so z has more digits than the inputs' type.  dz is rounded
+    to that type and dx = dz is not again: one half step of the slope, and what float32 leaves of it (F of
+    the terms whose sum it is, 20 of them at most, sigmoid's 1 - s being F e^|z| off)."""
+    from collie_amd import functional
+    a = torch.linspace(-9, 9, 4001).to(dtype)
+    b = (a.float().abs() * hb.U[dtype] * torch.rand(4001, generator=torch.Generator().manual_seed(1)))
+    x = torch.stack([a, b.to(dtype)], 1)
+    leaf, w = x.to(DEV).requires_grad_(), torch.ones(1, 2, dtype=dtype, device=DEV)
+    y = functional.linear(leaf, w, activation=kind)
+    (dx,) = torch.autograd.grad(y, [leaf], torch.ones_like(y))
+    z = x.double().sum(1)
+    _, slope, _, _ = hb.act(z, kind)
+    terms = 20 * F * (1 + z.abs()) if kind != 'sigmoid' else 20 * F * torch.sigmoid(z)
+    room = hb.U[dtype] * slope.abs() + terms + hb.TINY[dtype]
+    for col in range(2):
+        err = (dx[:, col].double().cpu() - slope).abs()
+        assert (err <= room).all(), (err / room).max()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('kind', ['relu', 'leaky_relu'])
+def test_slope_of_sums_below_the_range_of_the_type(kind, dtype):
+    """x w is positive and rounds to zero in float16: the slope is that of the positive side."""
+    from collie_amd import functional
+    small = {torch.float32: 2.0 ** -60, torch.bfloat16: 2.0 ** -60, torch.float16: 2.0 ** -14}[dtype]
+    x = torch.tensor([[small], [-small], [0.0]], dtype=dtype, device=DEV).requires_grad_()
+    w = torch.full((1, 1), small, dtype=dtype, device=DEV)
+    y = functional.linear(x, w, activation=kind)
+    (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    low = 0.0 if kind == 'relu' else torch.tensor(0.01).to(dtype).item() * small
+    want = torch.tensor([[small], [low], [low]]).to(dtype)
+    assert torch.equal(dx.cpu(), want)
