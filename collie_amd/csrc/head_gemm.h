@@ -36,7 +36,23 @@ struct Gemm {
   int64_t row_split;     // only the first row_valid are wanted
   int64_t row_valid;
   bool stream;           // the results are stored past the caches
+  const uint32_t* over;  // float16, kEpiStore: where not 0, a is kDzScale times what it stands for
 };
+
+// float16 ends at 65504, and an activation gradient (dy u f'(g) in the gated layer) may go past that
+// although its products with the weights do not.  Where any finite one of a call does, all are stored
+// times this power of two, and the products are divided by it again in float32.  Values below 2^-17 are
+// then rounded to multiples of it, so it is no smaller: what lies past 1.6e7 stays infinite.
+constexpr float kDzScale = 1.0f / 256.0f;
+constexpr float kHalfMax = 65504.0f;
+
+// what to multiply a result of this launch by
+template <typename T, int EPI>
+__device__ __forceinline__ float result_scale(const Gemm& g) {
+  if constexpr (EPI == kEpiStore && std::is_same<T, f16_t>::value)
+    if (g.over && *g.over) return 1.0f / kDzScale;
+  return 1.0f;
+}
 
 // biases of the columns col .. col + W
 template <typename T, int EPI, int W>
@@ -52,11 +68,16 @@ __device__ __forceinline__ void load_biases(const Gemm& g, int64_t col, float (&
 // results at (row, col .. col + W): columns of one row that one thread holds
 template <typename T, int EPI, int W>
 __device__ __forceinline__ void finish_row(const Gemm& g, int64_t row, int64_t col, float (&v)[W],
-                                           float (&u)[W], const float (&b)[W], const float (&b2)[W]) {
+                                           float (&u)[W], const float (&b)[W], const float (&b2)[W],
+                                           float scale) {
   if (row >= g.m || col >= g.n) return;
   const int left = g.n - col < W ? static_cast<int>(g.n - col) : W;
   const int64_t at = row * g.n + col;
   if constexpr (EPI == kEpiStore) {
+    if constexpr (std::is_same<T, f16_t>::value) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] *= scale;
+    }
     T* c = static_cast<T*>(row < g.row_split ? g.c : g.c2);
     const int64_t r = row < g.row_split ? row : row - g.row_split;
     if (c && r < g.row_valid) store_pack<T, W>(c + r * g.n + col, left, v, g.stream);

@@ -29,13 +29,21 @@ struct ActBwd {
   int64_t rows_per_part;
   int act;
   bool stream;             // dz is stored past the caches
+  uint32_t* over;          // float16 (or NULL): set where a finite value of dz is past the type's range,
+  bool again;              // and the second launch, which stores dz times kDzScale if it is set
 };
 constexpr int kActLanes = 32;
 constexpr int kActRows = kBlock / kActLanes;
 
+__device__ __forceinline__ bool past_half(float v) {
+  return fabsf(v) > kHalfMax && fabsf(v) < INFINITY;
+}
+
 template <typename T, bool PAIR>
 __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
   constexpr int V = kVec<T>;
+  constexpr bool HALF = std::is_same<T, f16_t>::value;
+  if (HALF && p.again && *p.over == 0) return;
   const int lane = threadIdx.x % kActLanes, ry = threadIdx.x / kActLanes;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * kActLanes + lane) * V;
   const int left = col < p.n ? (p.n - col < V ? static_cast<int>(p.n - col) : V) : 0;
@@ -44,6 +52,7 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
   float sum[V], sum2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = sum2[j] = 0.0f;
+  bool over = false;
   if (left > 0) {
     for (int64_t row = r0 + ry; row < r1; row += kActRows) {
       float dy[V], z[V], d[V], u[V];
@@ -67,6 +76,13 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
           dy[j] *= d[j];
         }
         sum[j] += dy[j];
+        if (HALF) {
+          over = over || past_half(dy[j]) || (PAIR && past_half(u[j]));
+          if (p.again) {
+            dy[j] *= kDzScale;
+            if (PAIR) u[j] *= kDzScale;
+          }
+        }
       }
       if (p.dz) {
         // up to the padded width: what lies past n_out is 0
@@ -78,6 +94,7 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
       }
     }
   }
+  if (HALF && p.over && !p.again && __any(over) && (threadIdx.x & (kWave - 1)) == 0) atomicOr(p.over, 1u);
   if (p.partial == nullptr && p.db == nullptr && p.db2 == nullptr) return;
   __shared__ float sh[kActRows][kActLanes * V];
 #pragma unroll
@@ -101,6 +118,8 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
     }
   }
 }
+
+__global__ void clear_word_kernel(uint32_t* word) { *word = 0; }
 
 // out[c] = sum over `count` partials of partial[k][c], c < width, in fixed order; columns from
 // `split` on belong to out2.  64 columns x 16 slices of the partials per workgroup.
@@ -374,6 +393,7 @@ struct BwdWs {
   void *dz, *x, *w, *w2;
   float* act_partial;
   float* partial;
+  uint32_t* over;
   size_t bytes;
 };
 
@@ -395,6 +415,7 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
   const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false, sizeof(T)));
   const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false, sizeof(T)));
   ws.partial = c.take<float>(a > b ? a : b);
+  ws.over = c.take<uint32_t>(1);
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;
 }
@@ -448,6 +469,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
   const int64_t half = padded<T>(n_out);
   const void* dz = dy;
   int64_t dz_ld = dy_ld;
+  const uint32_t* over = nullptr;
   const bool sums = db || db2;
   if (z || sums) {
     ActBwd p;
@@ -472,13 +494,27 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
       p.db2 = db2;
     }
     p.rows_per_part = (m + parts - 1) / parts;
+    // (|f'| is at most 1 but for silu and gelu)
+    if (std::is_same<T, f16_t>::value && z && (dx || dw || dw2) &&
+        (pair || act == COLLIE_ACT_SILU || act == COLLIE_ACT_GELU)) {
+      p.over = ws.over;
+      hipLaunchKernelGGL(clear_word_kernel, dim3(1), dim3(1), 0, stream, p.over);
+      if (check_launch("clear_word_kernel")) return -2;
+    }
     const int64_t cols = kActLanes * kVec<T>;
     const dim3 grid(static_cast<unsigned>((n_out + cols - 1) / cols), static_cast<unsigned>(parts));
-    if (pair)
-      hipLaunchKernelGGL((act_bwd_kernel<T, true>), grid, dim3(kBlock), 0, stream, p);
-    else
-      hipLaunchKernelGGL((act_bwd_kernel<T, false>), grid, dim3(kBlock), 0, stream, p);
+    auto* kernel = pair ? act_bwd_kernel<T, true> : act_bwd_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, stream, p);
     if (check_launch("act_bwd_kernel")) return -2;
+    over = p.over;
+    if (p.over) {
+      ActBwd again = p;
+      again.again = true;
+      again.partial = nullptr;
+      again.db = again.db2 = nullptr;
+      hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, stream, again);
+      if (check_launch("act_bwd_kernel")) return -2;
+    }
     if (p.partial) {
       if (const int rc = sum_partials<T>(ws.act_partial, parts, wide * n_out, n_out, db, db2, stream))
         return rc;
@@ -507,6 +543,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     g.n = n_in;
     g.k = pair ? half + n_out : n_out;
     g.c = dx;
+    g.over = over;
     g.row_split = g.row_valid = m;
     g.partial = ws.partial;
     const int rc = pair ? launch_tiles<T, true, false, kEpiStore, true>(g, stream)
@@ -524,6 +561,7 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     g.row_valid = n_out;
     g.c = dw;
     g.c2 = dw2;
+    g.over = over;
     g.partial = ws.partial;
     return launch_tiles<T, false, false, kEpiStore, false>(g, stream);
   }

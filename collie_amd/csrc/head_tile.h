@@ -406,6 +406,7 @@ __global__ __launch_bounds__(kWave* WM* WN, BN == 64 ? 3 : 2) void gemm_tile_ker
   constexpr int W = sizeof(T) == 4 ? 4 : 8;  // columns that a lane stores together
   constexpr int G = 4 * HALF / W;
 
+  const float scale = result_scale<T, EPI>(g);
   int64_t n = blockIdx.x;
   Work now = work_at(n);
   int cur = 0;
@@ -489,7 +490,7 @@ __global__ __launch_bounds__(kWave* WM* WN, BN == 64 ? 3 : 2) void gemm_tile_ker
           store_pack<float, W>(p, W, v);
           if (PAIR) store_pack<float, W>(p + BM * TN, W, u);
         } else {
-          finish_row<T, EPI, W>(g, now.row0 + lr, now.col0 + lc, v, u, b[k], b2[k]);
+          finish_row<T, EPI, W>(g, now.row0 + lr, now.col0 + lc, v, u, b[k], b2[k], scale);
         }
       }
     }
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(kWave* kSkinnyWaves) void gemm_skinny_kernel(const 
         if (PAIR) u[t] += sums[s][i][PAIR ? 1 : 0][lane][t];
       }
     }
-    finish_row<T, EPI, 4>(g, i * 16 + r, col0 + 4 * q, v, u, bias, bias2);
+    finish_row<T, EPI, 4>(g, i * 16 + r, col0 + 4 * q, v, u, bias, bias2, 1.0f);
   }
 }
 
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(kWave* SLICES) void gemm_finish_kernel(const Gemm g
     u[j] = sum[NB - 1][j];
   }
   load_biases<T, EPI, 4>(g, col, bias, bias2);
-  finish_row<T, EPI, 4>(g, row, col, v, u, bias, bias2);
+  finish_row<T, EPI, 4>(g, row, col, v, u, bias, bias2, result_scale<T, EPI>(g));
 }
 
 }  // namespace collie

@@ -131,3 +131,97 @@ def test_slope_of_sums_below_the_range_of_the_type(kind, dtype):
     low = 0.0 if kind == 'relu' else torch.tensor(0.01).to(dtype).item() * small
     want = torch.tensor([[small], [low], [low]]).to(dtype)
     assert torch.equal(dx.cpu(), want)
+
+
+# ---- float16: activation gradients past the type's range -------------------------------------------
+def gated_case(m, n_in, n_out, seed):
+    """Ordinary values, and in some rows |dy u f'(g)| up to 5e5 where the weights are small."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, n_in, generator=g) * 0.25
+    wg = torch.randn(n_out, n_in, generator=g) / 64
+    wu = torch.randn(n_out, n_in, generator=g) / 64
+    bg, bu = torch.randn(n_out, generator=g), torch.randn(n_out, generator=g)
+    dy = torch.randn(m, n_out, generator=g)
+    bu[0], dy[m // 2, 0], dy[-1, 0] = 700.0, 600.0, -600.0
+    return [t.half() for t in (x, wg, wu, bg, bu, dy)]
+
+
+def check_gated(kind, case, run):
+    x, wg, wu, bg, bu, dy = case
+    ref = hb.gated(*(t.double() for t in (x, wg, wu, bg, bu)), kind, dy.double(), torch.float16)
+    assert (dy.double() * (x.double() @ wu.double().T + bu.double())).abs().max() > 4e5
+    names = ('dx', 'dwg', 'dwu', 'dbg', 'dbu')
+    # stored times 1 / 256, a value is off by half of 2^-24 times 256, wherever it is
+    low = 2.0 ** -17
+    more = {'dx': low * (wg.double().abs().sum(0) + wu.double().abs().sum(0)).expand(len(x), -1),
+            'dwg': low * x.double().abs().sum(0).expand(len(wg), -1)}
+    more['dwu'] = more['dwg']
+    for name, g in zip(names, run):
+        val, bound = ref[name]
+        hb.check(g, val, bound + more.get(name, 0.0), torch.float16)
+    # (hb.check lets a value be infinite only where the exact one may round to that: 4.2e5 |x| in dwg's
+    # first row does for |x| > 0.156)
+    assert torch.isfinite(run[0]).all()
+
+
+OVER = [(2, 24, 40), (70, 33, 130), (5000, 64, 48), (300, 520, 264)]
+
+
+@pytest.mark.parametrize('kind', ['identity', 'silu', 'leaky_relu'])
+@pytest.mark.parametrize('m,n_in,n_out', OVER)
+def test_float16_gated_gradients_past_the_range(m, n_in, n_out, kind):
+    from collie_amd import functional
+    case = gated_case(m, n_in, n_out, m)
+    leaves = [t.to(DEV).requires_grad_() for t in case[:5]]
+    y = functional.gated_linear(*leaves, activation=kind)
+    grads = torch.autograd.grad(y, leaves, case[5].to(DEV), retain_graph=True)
+    check_gated(kind, case, grads)
+    # a call in range afterwards is what it was before: nothing is kept
+    small = (case[5] / 1024).to(DEV)
+    first = torch.autograd.grad(y, leaves, small, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, case[5].to(DEV), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, small)))
+
+
+@pytest.mark.parametrize('kind', ['silu', 'gelu'])
+def test_float16_linear_gradients_past_the_range(kind):
+    """The slopes of silu and gelu go past one."""
+    from collie_amd import functional
+    x = torch.tensor([[2.0, 0.5], [1.4, 0.25]]).half()
+    w, dy = torch.tensor([[1.0, 1 / 64]]).half() / 2, torch.tensor([[65000.0], [-65000.0]]).half()
+    x[:, 0] = 2.4 * 2 if kind == 'silu' else 1.4 * 2
+    leaves = [x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()]
+    y = functional.linear(*leaves, activation=kind)
+    dx, dw = torch.autograd.grad(y, leaves, dy.to(DEV))
+    ref = hb.linear(x.double(), w.double(), None, None, kind, dy.double(), torch.float16)
+    assert (dy.double() * hb.act(x.double() @ w.double().T, kind)[1]).abs().min() > 65600
+    hb.check(dx, *ref['dx'], torch.float16)
+    hb.check(dw, *ref['dw'], torch.float16)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+
+
+def test_float16_gradients_past_the_range_in_a_captured_pass():
+    from collie_amd import functional
+    case = gated_case(70, 33, 130, 3)
+    leaves = [t.to(DEV).requires_grad_() for t in case[:5]]
+    dy = case[5].to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(functional.gated_linear(*leaves), leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(functional.gated_linear(*leaves), leaves, dy)
+    for factor in (1 / 1024, 1.0, 1 / 1024, 1.0):       # in range and past it, in turn
+        dy.copy_((case[5].float() * factor).half().to(DEV))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        eager = torch.autograd.grad(functional.gated_linear(*leaves), leaves, dy)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+        if factor == 1.0:
+            check_gated('silu', case, got)
