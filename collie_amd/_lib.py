@@ -256,6 +256,8 @@ SIGNATURES = {
     'collie_layer_backward_workspace_bytes': (c_size_t, [c_void_p, c_int64, c_void_p, c_int64,
                                                          c_int32, c_int64, c_int32, c_void_p,
                                                          c_void_p, c_int32, c_int32]),
+    'collie_layer_plan': (ctypes.c_int, [c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+                                         POINTER(c_int64)]),
     'collie_linear_forward': (ctypes.c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
                                              c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
                                              c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -47,6 +47,21 @@ extern "C" size_t collie_layer_backward_workspace_bytes(const void* dy, int64_t 
   return bytes;
 }
 
+extern "C" int collie_layer_plan(int32_t dtype, int32_t product, int32_t gated, int64_t m, int32_t n_in,
+                                 int32_t n_out, int64_t* plan) {
+  if (check_layer("layer_plan", m, n_in, n_out, n_in, COLLIE_ACT_IDENTITY)) return -1;
+  COLLIE_REQUIRE(m >= 1 && plan, "layer_plan: no rows or no room for the plan");
+  COLLIE_REQUIRE(product >= COLLIE_PRODUCT_FORWARD && product <= COLLIE_PRODUCT_DW,
+                 "layer_plan: unknown product %d", product);
+  return with_type(dtype, "layer_plan", [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    int64_t out[5];
+    HeadLayer<T>::plan(static_cast<Product>(product), m, n_in, n_out, gated != 0, out);
+    memcpy(plan, out, sizeof(out));
+    return 0;
+  });
+}
+
 extern "C" int collie_linear_forward(const void* x, int64_t x_ld, int32_t dtype, int64_t m,
                                      int32_t n_in, const void* weight, const void* bias,
                                      int32_t n_out, int32_t act, const void* residual,

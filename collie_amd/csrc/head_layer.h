@@ -6,8 +6,12 @@
 
 namespace collie {
 
+enum Product { kForward = COLLIE_PRODUCT_FORWARD, kDx = COLLIE_PRODUCT_DX, kDw = COLLIE_PRODUCT_DW };
+
 template <typename T>
 struct HeadLayer {
+  static void plan(Product product, int64_t m, int64_t n_in, int64_t n_out, bool pair,
+                   int64_t (&out)[5]);
   static size_t forward_bytes(const void* x, int64_t x_ld, int64_t m, int64_t n_in, const void* w,
                               const void* w2, int64_t n_out);
   static size_t backward_bytes(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int64_t m,

@@ -299,6 +299,17 @@ double stored_bytes(bool pair) {
   return pair ? (sizeof(T) + 8.0) / 2 : 2.0 * sizeof(T);
 }
 
+// the products of a layer: x W^T, dz W (gated: over [dg | du] in one) and dz^T x (the columns of [dg | du])
+template <typename T>
+Plan plan_of(Product product, int64_t m, int64_t n_in, int64_t n_out, bool pair) {
+  const int64_t both = pair ? padded<T>(n_out) + n_out : n_out;
+  switch (product) {
+    case kForward: return plan_gemm<T>(m, n_out, n_in, pair, stored_bytes<T>(pair));
+    case kDx: return plan_gemm<T>(m, n_in, both, false, sizeof(T));
+    default: return plan_gemm<T>(both, n_in, m, false, sizeof(T));
+  }
+}
+
 size_t partial_floats(const Plan& p) {
   return static_cast<size_t>(p.splits > 1 ? p.splits * (p.tiles - p.full) * p.bm * p.bn : 0);
 }
@@ -322,9 +333,7 @@ int launch_tile(const Gemm& g, const Plan& p, hipStream_t stream) {
 }
 
 template <typename T, bool AKC, bool BKC, int EPI, bool CAT>
-int launch_tiles(Gemm& g, hipStream_t stream) {
-  constexpr bool PAIR = EPI == kEpiGated;
-  const Plan p = plan_gemm<T>(g.m, g.n, g.k, PAIR, EPI == kEpiStore ? sizeof(T) : stored_bytes<T>(PAIR));
+int launch_tiles(Gemm& g, const Plan& p, hipStream_t stream) {
   g.stream = g.m * g.n * static_cast<int64_t>(sizeof(T)) >= kStreamBytes;
   g.full = p.full;
   g.splits = static_cast<int>(p.splits);
@@ -382,8 +391,7 @@ FwdWs carve_fwd(void* base, const void* x, int64_t x_ld, int64_t m, int64_t n_in
     if (!whole_packs<T>(x, x_ld, n_in)) ws.x = c.take<T>(m * wide);
     if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
     if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
-    ws.partial = c.take<float>(partial_floats(
-        plan_gemm<T>(m, n_out, n_in, w2 != nullptr, stored_bytes<T>(w2 != nullptr))));
+    ws.partial = c.take<float>(partial_floats(plan_of<T>(kForward, m, n_in, n_out, w2 != nullptr)));
   }
   ws.bytes = align_up(c.off, 256) + 256;
   return ws;
@@ -412,8 +420,8 @@ BwdWs carve_bwd(void* base, const void* dy, int64_t dy_ld, const void* x, int64_
   if (!whole_packs<T>(w, n_in, n_in)) ws.w = c.take<T>(n_out * wide);
   if (w2 && !whole_packs<T>(w2, n_in, n_in)) ws.w2 = c.take<T>(n_out * wide);
   ws.act_partial = c.take<float>(static_cast<size_t>(act_parts(m, n_out, kVec<T>)) * pair * n_out);
-  const size_t a = partial_floats(plan_gemm<T>(m, n_in, (pair - 1) * half + n_out, false, sizeof(T)));
-  const size_t b = partial_floats(plan_gemm<T>((pair - 1) * half + n_out, n_in, m, false, sizeof(T)));
+  const size_t a = partial_floats(plan_of<T>(kDx, m, n_in, n_out, w2 != nullptr));
+  const size_t b = partial_floats(plan_of<T>(kDw, m, n_in, n_out, w2 != nullptr));
   ws.partial = c.take<float>(a > b ? a : b);
   ws.over = c.take<uint32_t>(1);
   ws.bytes = align_up(c.off, 256) + 256;
@@ -454,8 +462,9 @@ int layer_forward(const void* x, int64_t x_ld, const void* w, const void* w2, co
   g.b2 = w2;
   if (m <= kSkinnyRows)
     return w2 ? launch_skinny<T, kEpiGated>(g, stream) : launch_skinny<T, kEpiLinear>(g, stream);
-  return w2 ? launch_tiles<T, true, true, kEpiGated, false>(g, stream)
-            : launch_tiles<T, true, true, kEpiLinear, false>(g, stream);
+  const Plan p = plan_of<T>(kForward, m, n_in, n_out, w2 != nullptr);
+  return w2 ? launch_tiles<T, true, true, kEpiGated, false>(g, p, stream)
+            : launch_tiles<T, true, true, kEpiLinear, false>(g, p, stream);
 }
 
 template <typename T>
@@ -546,8 +555,9 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     g.over = over;
     g.row_split = g.row_valid = m;
     g.partial = ws.partial;
-    const int rc = pair ? launch_tiles<T, true, false, kEpiStore, true>(g, stream)
-                        : launch_tiles<T, true, false, kEpiStore, false>(g, stream);
+    const Plan p = plan_of<T>(kDx, m, n_in, n_out, pair);
+    const int rc = pair ? launch_tiles<T, true, false, kEpiStore, true>(g, p, stream)
+                        : launch_tiles<T, true, false, kEpiStore, false>(g, p, stream);
     if (rc) return rc;
   }
   if (dw || dw2) {
@@ -563,7 +573,8 @@ int layer_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, c
     g.c2 = dw2;
     g.over = over;
     g.partial = ws.partial;
-    return launch_tiles<T, false, false, kEpiStore, false>(g, stream);
+    return launch_tiles<T, false, false, kEpiStore, false>(
+        g, plan_of<T>(kDw, m, n_in, n_out, pair), stream);
   }
   return 0;
 }
@@ -581,6 +592,18 @@ size_t HeadLayer<T>::backward_bytes(const void* dy, int64_t dy_ld, const void* x
                                     int64_t m, int64_t n_in, const void* w, const void* w2,
                                     int64_t n_out, int act) {
   return carve_bwd<T>(nullptr, dy, dy_ld, x, x_ld, m, n_in, w, w2, n_out, act).bytes;
+}
+
+template <typename T>
+void HeadLayer<T>::plan(Product product, int64_t m, int64_t n_in, int64_t n_out, bool pair,
+                        int64_t (&out)[5]) {
+  if (product == kForward && m <= kSkinnyRows) {
+    memset(out, 0, sizeof(out));
+    return;
+  }
+  const Plan p = plan_of<T>(product, m, n_in, n_out, pair);
+  const int64_t values[5] = {p.bm, p.bn, p.tiles, p.full, p.splits};
+  memcpy(out, values, sizeof(out));
 }
 
 template <typename T>

@@ -864,6 +864,13 @@ size_t collie_layer_backward_workspace_bytes(const void* dy, int64_t dy_ld, cons
                                              const void* weight, const void* up_weight,
                                              int32_t n_out, int32_t act);
 
+/* Which tiles one of a layer's products takes, into plan[5] (host only): rows and columns of a tile (0:
+ * no tiles, the kernel that streams the weights), number of tiles, how many of them are computed whole,
+ * and into how many parts of the depth each of the others is cut. */
+enum { COLLIE_PRODUCT_FORWARD = 0, COLLIE_PRODUCT_DX = 1, COLLIE_PRODUCT_DW = 2 };
+int collie_layer_plan(int32_t dtype, int32_t product, int32_t gated, int64_t m, int32_t n_in,
+                      int32_t n_out, int64_t* plan);
+
 /* y = act(x weight^T + bias) + residual ([m, n_out]); weight [n_out, n_in]; bias / residual may be
  * NULL.  keep [m, n_out] (NULL: not wanted) takes the pre-activations for the backward pass: float32
  * for sigmoid, silu and gelu; for relu and leaky_relu in x's type, where only the sign is kept to the
