@@ -38,7 +38,8 @@ class Table(torch.nn.Embedding):
         if self._status is None or self._status.device != self.weight.device:
             if torch.cuda.is_current_stream_capturing():
                 return None     # memory of the graph, which would clear it with every replay
-            self._status = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
+            with torch.inference_mode(False):       # (check_status writes to it outside of that mode)
+                self._status = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
         return self._status
 
     @torch.jit.unused

@@ -175,3 +175,15 @@ def test_a_table_captured_before_its_first_call():
         graph.replay()
         assert torch.equal(y, t.weight[ids])
         torch.cuda.synchronize()
+
+
+def test_a_table_first_called_in_inference_mode():
+    from collie_amd import layers
+    t = layers.ScaledEmbedding(5, 3).to(DEV)
+    with torch.inference_mode():
+        y = t(torch.tensor([1, 7], device=DEV))
+    assert torch.equal(y[1], torch.zeros(3, device=DEV))
+    for _ in range(2):
+        with pytest.raises(IndexError):
+            t.check_status()
+        t(torch.tensor([-1], device=DEV))
