@@ -65,8 +65,9 @@ struct Frag<float> {
 // weight 2^-16 and more are summed; the others are below 2^-23 of the product, which is what float32
 // rounds it by.  Six bfloat16 instructions do 32 k in 96 cycles; the float32 ones need 256.  Values
 // without a finite bfloat16 (infinities, NaN, the top of the range) make sums that are not finite:
-// the tile is then computed again with the float32 instructions (gemm_tile_kernel).  Parts below the
-// smallest normal number are lost, at most 2^-126 times the other factor.
+// the tile is then computed again with the float32 instructions (gemm_tile_kernel).  Parts end at
+// bfloat16's smallest number: at most 2^-134 times the other factor is lost, which is float32's own
+// rounding down to 2^-110.
 struct Split {
   bf16x8 hi, mid, lo;
 };

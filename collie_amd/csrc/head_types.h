@@ -128,6 +128,4 @@ int with_type(int32_t dtype, const char* who, F&& f) {
   }
 }
 
-inline size_t type_size(int32_t dtype) { return dtype == COLLIE_F32 ? 4 : 2; }
-
 }  // namespace collie

@@ -4,12 +4,20 @@ embedding rows with scaling, layer normalisation, the linear layer with bias, ac
 residual, and the gated layer.  ``collie_amd.layers`` has them as modules.
 
 Inputs are float32, bfloat16 or float16 (all of one call alike; under ``torch.autocast`` the caller
-casts); sums, statistics and activations are computed in float32 and every result is rounded once.
-Gradients are summed in a fixed order: equal calls give equal bits.  Layers other than the embedding
-rows can be differentiated once.  There is no CPU fallback.  What torch records or transforms by its
-own calls does not see these: tensors under ``vmap``, ``torch.func`` or ``torch.jit.trace``, fake
-tensors and forward-mode tangents are refused (the tables of ``collie_amd.layers``, called as modules,
-then do what ``torch.nn.Embedding`` does).
+casts); sums, statistics and activations are computed in float32 and every result of a forward pass is
+rounded once.  Gradients are summed in a fixed order: equal calls give equal bits.  Layers other than
+the embedding rows can be differentiated once.
+
+Three things are not as float32 would have them.  In bfloat16 and float16 the gradient before an
+activation (``dy f'(z)``; of the gated layer both) is rounded to the type before it is multiplied with
+the weights and the inputs, so their gradients are 1.4 times one rounding off; in float16 a part of it
+below 2^-25 is lost and one past 1.6e7 is infinite (the bias gradients are sums of the unrounded ones).
+In float32, matrix products are made of bfloat16 ones, exact to float32's own rounding for magnitudes
+from about 2^-110 up; smaller values keep fewer digits.
+
+There is no CPU fallback.  What torch records or transforms by its own calls does not see these: tensors
+under ``vmap``, ``torch.func`` or ``torch.jit.trace``, fake tensors and forward-mode tangents are refused
+(the tables of ``collie_amd.layers``, called as modules, then do what ``torch.nn.Embedding`` does).
 
 Everything is launched on the current stream of the inputs' device and can be captured into a graph.
 As with any torch operation, drop eager results that depend on the same leaves before a backward pass

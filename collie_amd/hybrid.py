@@ -141,7 +141,7 @@ class HybridPretrainedModel(MatrixFactorizationModel):
     Parameters are those of the reference (``hybrid_pretrained_matrix_factorization.py:102-126``):
     ``train, val, item_metadata, user_metadata, trained_model, item_metadata_layers_dims,
     user_metadata_layers_dims, combined_layers_dims=[128, 64, 32], freeze_embeddings=True,
-dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', loss='hinge',
+    dropout_p=0.0, lr=1e-3, lr_scheduler_func, weight_decay=0.0, optimizer='adam', loss='hinge',
     metadata_for_loss, metadata_for_loss_weights, load_model_path, map_location``.
 
     One more, ``combined_blocks`` (0: the reference's head), makes the head deeper: that many residual

@@ -807,7 +807,9 @@ int collie_dense_rows_update(float* table, int64_t num_rows, int32_t dim, const 
 /* ---- layers of a deeper ranking head -----------------------------------------------------------
  * Embedding rows with scaling, layer normalisation, the linear layer with bias, activation and
  * residual, and the gated layer, each with its gradient.  Values are float32, bfloat16 or float16
- * (COLLIE_F32 / COLLIE_BF16 / COLLIE_F16), sums and statistics float32; a result is rounded once.
+ * (COLLIE_F32 / COLLIE_BF16 / COLLIE_F16), sums and statistics float32; a result is rounded once, and the
+ * gradients of 16-bit layers come from a dz (dg, du) that was rounded to the type as well: float16 keeps
+ * none of it below 2^-25 and none past 1.6e7.
  * (float32 matrix products are made of bfloat16 ones, exact to float32's own rounding for magnitudes
  * from about 2^-110 up; smaller values keep fewer digits.)
  * Rows may be apart by more than their width (`*_ld`, in elements, >= the width); tables, weights,

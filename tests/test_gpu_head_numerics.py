@@ -251,3 +251,18 @@ def test_gradients_are_two_roundings_off_in_the_mean(gated, dtype):
         ratio = ((grad.cpu().double() - want).norm() / one).item()
         print(name, ratio)
         assert ratio < 1.6, (name, ratio)
+
+
+def test_float32_products_of_small_values():
+    """A value is split into three bfloat16 parts, the last a multiple of 2^-133: off by half of that, and by
+    nothing from 2^-110 on (24 bits reach 2^-133).  One column, weights powers of two: no other rounding
+    but that of results below 2^-126."""
+    from collie_amd import functional
+    g = torch.Generator().manual_seed(2)
+    e = torch.arange(-126, -60).repeat_interleave(8)
+    x = torch.ldexp(1 + torch.rand(len(e), generator=g), e)[:, None]
+    for power in (0, 20):
+        y = functional.linear(x.to(DEV), torch.full((70, 1), 2.0 ** power, device=DEV)).cpu().double()
+        want = x.double() * 2.0 ** power
+        lost = torch.where(e[:, None] < -110, 2.0 ** -134, 0.0).double() * 2.0 ** power
+        assert ((y - want).abs() <= lost).all()
