@@ -52,7 +52,7 @@ def table_grad(table, ids, vals, status=None):
     take no gradient (the lookup has set bit 0 of ``status`` for them)."""
     rows = table.shape[0]
     vals = vals.reshape(ids.shape[0], table.shape[1])
-    if ids.shape[0] < SORTED_GRAD_ROWS:
+    if not SORTED_GRAD_ROWS <= ids.shape[0] < 1 << 30:     # (the sorted form ends there)
         # index_add_ does not look at the ids on every build of torch: those outside the table (-1 and
         # `rows` after the clamp, `rows` after the remainder) go to a row behind it
         inside = ids.long().clamp(-1, rows).remainder_(rows + 1)

@@ -53,13 +53,15 @@ class Table(torch.nn.Embedding):
 
     @torch.jit.unused
     def _kernels_take(self, input) -> bool:
-        # What the kernels do not take stays torch's: other devices and types, empty tables,
-        # renormalised rows, gradients divided by counts; and calls that stand for others (recorded,
-        # compiled or transformed ones, tensors with forward-mode tangents).
+        # What the kernels do not take stays torch's: other devices and types, empty tables and those
+        # past the entry points' limits, renormalised rows, gradients divided by counts; and calls that
+        # stand for others (recorded, compiled or transformed ones, tensors with forward-mode tangents).
         if (torch.compiler.is_compiling() or torch.jit.is_tracing()
                 or torch.overrides.has_torch_function((input, self.weight))):
             return False
         return (self.weight.is_cuda and self.weight.numel() > 0
+                and self.weight.shape[0] < (1 << 31) - 1 and self.weight.shape[1] <= 1 << 20
+                and input.numel() < 1 << 30
                 and self.weight.dtype in _lib.ELEMENT_TYPES
                 and input.is_cuda and input.dtype in (torch.int32, torch.int64)
                 and self.max_norm is None and not self.scale_grad_by_freq

@@ -187,3 +187,28 @@ def test_a_table_first_called_in_inference_mode():
         with pytest.raises(IndexError):
             t.check_status()
         t(torch.tensor([-1], device=DEV))
+
+
+def test_tables_past_the_limits_of_the_entry_points_are_torch_s():
+    t = _table(rows=2, dim=(1 << 20) + 1)
+    ids = torch.tensor([1, 0, 1], device=DEV)
+    y = t(ids)
+    assert torch.equal(y, t.weight[ids])
+    y.sum().backward()
+    assert torch.equal(t.weight.grad[:, :2].cpu(), torch.tensor([[1.0, 1.0], [2.0, 2.0]]))
+
+
+def test_layers_inside_a_compiled_function():
+    """The compiler breaks its graph at the functions and calls them as they are."""
+    from collie_amd import functional as F
+    w = torch.randn(6, 4, generator=torch.Generator().manual_seed(0)).to(DEV).requires_grad_()
+    x = torch.randn(9, 4, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    def f(x, w):
+        return F.linear(F.layer_norm(x * 2.0), w, activation='silu') + 1.0
+
+    got = torch.compile(f, backend='eager')(x, w)
+    want = f(x, w)
+    assert torch.equal(got, want)
+    (a,), (b,) = (torch.autograd.grad(y.sum(), [w]) for y in (got, want))
+    assert torch.equal(a, b)
